@@ -309,6 +309,103 @@ KVOFF_API int kvoff_store_kvcache(const void* key, int64_t key_stride_bytes, con
                                   int64_t num_tokens, int64_t num_slots, int32_t* bad_slots,
                                   void* stream);
 
+/* Types of rows that are not moved byte for byte. */
+enum kvoff_dtype { KVOFF_BF16 = 0, KVOFF_FP16 = 1, KVOFF_FP32 = 2 };
+
+/*
+ * Rotary positions of q [num_tokens, q_heads, head_dim] and k [num_tokens,
+ * kv_heads, head_dim] (heads dense, tokens strided; bf16, fp16 or fp32):
+ *     y1 = x1 * cos - x2 * sin,  y2 = x2 * cos + x1 * sin
+ * for the rotary_dim / 2 pairs of each head, (x_j, x_{j + rotary_dim/2}), or
+ * (x_2j, x_2j+1) with KVOFF_ROTARY_INTERLEAVED; values from rotary_dim on pass
+ * through. Row p of `table` [table_rows, rotary_dim] (fp32) holds position p's
+ * cosines, then its sines. KVOFF_ROTARY_INVERSE applies the transposed map
+ * (the gradient). Products are fp32, rounded once. q_out and k_out may be q
+ * and k (in place) but must not overlap them otherwise. A token whose position
+ * is negative is skipped: nothing of it is written; one whose position is not
+ * in the table is skipped and counted into *bad_positions when that is
+ * non-null (device memory). Enqueues one kernel, allocates nothing.
+ */
+enum kvoff_rotary_flags { KVOFF_ROTARY_INTERLEAVED = 1, KVOFF_ROTARY_INVERSE = 2 };
+KVOFF_API int kvoff_rotary(const void* q, int64_t q_stride_bytes, void* q_out,
+                           int64_t q_out_stride_bytes, int64_t q_heads, const void* k,
+                           int64_t k_stride_bytes, void* k_out, int64_t k_out_stride_bytes,
+                           int64_t kv_heads, int64_t head_dim, int64_t rotary_dim, int32_t dtype,
+                           const void* positions, int32_t position_bytes, const float* table,
+                           int64_t table_rows, int64_t num_tokens, int32_t flags,
+                           int32_t* bad_positions, void* stream);
+
+/*
+ * Slot-mapping scatter of fresh K/V rows [num_tokens, num_heads, head_dim]
+ * (bf16 or fp16) into an e4m3 paged cache [pages, page, num_heads, head_dim]
+ * with one fp32 scale for each block of scale_block tokens (a power of two
+ * that divides the page) and head, [pages, page / scale_block, num_heads]:
+ *     scale   = the smallest 2^e (e >= -100) with amax <= 448 * 2^e over the
+ *               block's finite values
+ *     payload = e4m3_rne(x / scale), NaN where x is not finite
+ * A call that writes a block's first token opens the block: its old scale and
+ * rows no longer count, and rows that the call does not write keep their
+ * bytes. Otherwise the scale only grows (an old one that is not positive and
+ * finite counts as zero), and the block's other rows are multiplied by old /
+ * new scale and rounded again, exact but for e4m3's subnormals. Slots come in
+ * any order; of a slot that occurs twice the later row stays. Negative slots
+ * are skipped; slots >= num_slots are skipped and counted into *bad_slots when
+ * it is non-null (device memory). At most 65536 tokens a call. head_dim is a
+ * multiple of 8 up to 256; rows are 16-byte aligned, caches 8-byte. Enqueues
+ * one kernel, allocates nothing.
+ */
+KVOFF_API int kvoff_store_kvcache_fp8(const void* key, int64_t key_stride_bytes,
+                                      const void* value, int64_t value_stride_bytes,
+                                      void* k_cache, void* v_cache, float* k_scale,
+                                      float* v_scale, int64_t num_heads, int64_t head_dim,
+                                      int32_t dtype, int64_t scale_block,
+                                      const int32_t* slot_mapping, int64_t num_tokens,
+                                      int64_t num_slots, int32_t* bad_slots, void* stream);
+
+/*
+ * Causal attention of q [num_tokens, q_heads, head_dim] (bf16 or fp16, heads
+ * dense, tokens strided) over an e4m3 paged cache as kvoff_store_kvcache_fp8
+ * writes it:
+ *     out = softmax(softmax_scale * q . k_t) . v_t,  k, v = payload * scale
+ * Sequence s has the keys 0 .. context_lens[s] - 1 (its new tokens included,
+ * at the end) in the pages block_tables[s * table_stride ...], and the query
+ * tokens cu_seqlens_q[s] .. cu_seqlens_q[s + 1] - 1 (NULL: token s alone);
+ * query token t of n sees the keys below context - n + t + 1. A row that sees
+ * none is 0 (lse -inf). lse, when non-null, receives each row's log-sum-exp
+ * [num_tokens, q_heads] (natural logarithm). Each KV head serves q_heads /
+ * kv_heads query heads. Scales are finite and not negative; they may be any
+ * such numbers, not only powers of two.
+ *
+ * A page id that is negative or not below num_pages is not read: its keys
+ * count as absent. A context longer than the table is cut to it; offsets of
+ * cu_seqlens_q are cut to num_tokens. Tokens of q that belong to no sequence
+ * leave their rows of out and lse as they were. max_seqlen_q is the longest
+ * query length (it sizes the launch; the lengths themselves stay on the
+ * device). Values in keys that a row does not see, NaN among them, do not
+ * reach it.
+ *
+ * head_dim is 64 or 128, page_size a multiple of 16, scale_block 16 * 2^n
+ * tokens and a divisor of the page; q and the caches are 16-byte aligned.
+ * workspace: device memory of at least kvoff_attention_fp8_workspace bytes
+ * (16-byte aligned), whose contents mean nothing before and after; calls that
+ * may run at the same time need one each. Allocates nothing and reads no
+ * device value on the host, so it can be captured in a CUDA graph.
+ */
+KVOFF_API int kvoff_attention_fp8(
+    const void* q, int64_t q_stride_bytes, void* out, int64_t out_stride_bytes, float* lse,
+    const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+    int64_t num_pages, int64_t page_size, int64_t scale_block, const int32_t* block_tables,
+    int64_t table_stride, int64_t table_width, const int32_t* context_lens,
+    const int32_t* cu_seqlens_q, int64_t num_seqs, int64_t num_tokens, int64_t max_seqlen_q,
+    int64_t q_heads, int64_t kv_heads, int64_t head_dim, int32_t dtype, float softmax_scale,
+    void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes of a kvoff_attention_fp8 call of these sizes on the current device. */
+KVOFF_API int kvoff_attention_fp8_workspace(int64_t num_seqs, int64_t max_seqlen_q,
+                                            int64_t table_width, int64_t page_size,
+                                            int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                            int64_t* bytes);
+
 /*
  * Pinned host slab: mmap `bytes`, prefer NUMA node `numa_node` (-1: no
  * preference), page-lock it with cudaHostRegister(Portable | Mapped) and

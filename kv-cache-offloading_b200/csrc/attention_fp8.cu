@@ -1,0 +1,219 @@
+// Entry points of attention over the e4m3 paged cache, and the join of rows
+// whose keys were read by several CTAs.
+#include "attention_fp8.h"
+
+namespace kvoff {
+namespace attention {
+namespace {
+
+constexpr int kJoinThreads = 256;
+
+// Every record's CTA joins the split row tile that begins in that CTA of the
+// attention kernel: o = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c over its
+// parts, in the order of their keys, so the result does not depend on timing.
+// A warp takes a row; blockIdx.y picks 64 values of it.
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Args a, int dim) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the parts are complete
+  const int first = blockIdx.x;
+  const Record record = a.records[first];
+  if (record.further < 0) return;
+  Sequence seq;
+  seq.load(a, record.seq);
+  const int rows = min(a.rows, seq.q_len * a.group - record.tile * a.rows);
+  const int lane = threadIdx.x % 32, d = blockIdx.y * 64 + lane * 2;
+  const int64_t slot = slot_floats(a.rows, dim);
+  for (int row = threadIdx.x / 32 + blockIdx.z * (kJoinThreads / 32); row < rows;
+       row += kJoinThreads / 32 * gridDim.z) {
+    float most = __int_as_float(0xFF800000), l = 0.0f;
+    float2 sum = make_float2(0.0f, 0.0f);
+    bool any = false;
+    auto part = [&](int cta, int which) {
+      const float* p = a.partial + ((int64_t)cta * 2 + which) * slot;
+      const float m = p[a.rows * dim + row], part_l = p[a.rows * dim + a.rows + row];
+      const float2 x = *reinterpret_cast<const float2*>(p + row * dim + d);
+      any = true;
+      const float top = fmaxf(most, m);
+      if (top == __int_as_float(0xFF800000)) {  // no key seen: o is 0, or NaN from NaN scores
+        sum.x += x.x, sum.y += x.y, l += part_l;
+        return;
+      }
+      const float keep = exp2_fast(most - top), take = exp2_fast(m - top);
+      sum.x = sum.x * keep + x.x * take;
+      sum.y = sum.y * keep + x.y * take;
+      l = l * keep + part_l * take;
+      most = top;
+    };
+    if (record.valid[1]) part(first, 1);
+    for (int c = first + 1; c <= first + record.further; ++c)
+      if (a.records[c].valid[0]) part(c, 0);
+    if (!any) continue;  // one CTA had all of it and wrote the result
+    const int at = record.tile * a.rows + row;
+    const int token = seq.start + at / a.group, head = record.head * a.group + at % a.group;
+    const float scale = l == 0.0f ? 0.0f : 1.0f / l;
+    write_pair(a, token, head, dim, d, sum.x * scale, sum.y * scale);
+    if (d == 0) write_lse(a, token, head, most, l);
+  }
+}
+
+}  // namespace
+
+int launch_join(const Args& a, int dim, int grid, cudaStream_t stream) {
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(grid, dim / 64, a.rows > 32 ? 8 : 1);
+  config.blockDim = dim3(kJoinThreads);
+  config.stream = stream;
+  cudaLaunchAttribute attribute[1];
+  attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute[0].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attribute;
+  config.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&config, join_kernel, a, dim), "attention_fp8 join launch");
+}
+
+namespace {
+
+// Longest context (in keys) that one CTA reads alone rather than sharing it:
+// the join is a second launch.
+constexpr int64_t kDirectKeys = 1024;
+
+struct Shape {
+  int64_t seqs, max_q, keys, q_heads, kv_heads, dim;
+};
+
+// How a call is launched: rows of a tile, CTAs, and whether rows are split.
+struct Choice {
+  int rows, grid;
+  int64_t max_tiles;
+  bool direct;
+};
+
+Choice choose(const Shape& s) {
+  Choice c{};
+  const int64_t rows = s.max_q * (s.q_heads / s.kv_heads);
+  c.rows = decode_rows(rows);
+  c.max_tiles = (rows + c.rows - 1) / c.rows;
+  const int64_t ctas = s.seqs * s.kv_heads * c.max_tiles;
+  c.direct = s.keys <= kDirectKeys && ctas <= 0x7FFFFFFFll;
+  c.grid = c.direct ? (int)ctas : decode_grid();
+  return c;
+}
+
+int64_t workspace_of(const Choice& c, int64_t dim) {
+  if (c.direct) return 0;
+  return c.grid * ((int64_t)sizeof(Record) + 2 * slot_floats(c.rows, (int)dim) * (int64_t)sizeof(float));
+}
+
+int check_shape(const Shape& s, int64_t page) {
+  if (s.seqs < 0 || s.max_q < 0 || s.keys < 0 || s.q_heads <= 0 || s.kv_heads <= 0 || page <= 0)
+    return fail(KVOFF_EINVAL, "kvoff_attention_fp8: bad sizes");
+  if (s.dim != 64 && s.dim != 128)
+    return fail(KVOFF_EINVAL, "kvoff_attention_fp8: head_dim %lld is not 64 or 128",
+                (long long)s.dim);
+  if (s.q_heads % s.kv_heads != 0 || s.q_heads > 65535)
+    return fail(KVOFF_EINVAL, "kvoff_attention_fp8: %lld query heads do not divide over %lld KV heads",
+                (long long)s.q_heads, (long long)s.kv_heads);
+  if (page % 16 != 0)
+    return fail(KVOFF_EINVAL, "kvoff_attention_fp8: page size %lld is not a multiple of 16",
+                (long long)page);
+  if (s.seqs > 0x7FFFFFFFll || s.keys > 0x7FFFFF00ll || s.max_q > 0x7FFFFFFFll / s.q_heads)
+    return fail(KVOFF_EINVAL, "kvoff_attention_fp8: sizes exceed 32 bits");
+  return KVOFF_OK;
+}
+
+}  // namespace
+}  // namespace attention
+}  // namespace kvoff
+
+using namespace kvoff;
+
+extern "C" int kvoff_attention_fp8_workspace(int64_t num_seqs, int64_t max_seqlen_q,
+                                             int64_t table_width, int64_t page_size,
+                                             int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                             int64_t* bytes) {
+  if (bytes == nullptr) return fail(KVOFF_EINVAL, "kvoff_attention_fp8_workspace: null output");
+  if (table_width < 0 || (page_size > 0 && table_width > 0x7FFFFF00ll / page_size))
+    return fail(KVOFF_EINVAL, "kvoff_attention_fp8: sizes exceed 32 bits");
+  const attention::Shape s{num_seqs, max_seqlen_q, table_width * page_size, q_heads, kv_heads, head_dim};
+  KVOFF_TRY(attention::check_shape(s, page_size));
+  *bytes = attention::workspace_of(attention::choose(s), head_dim);
+  return ok();
+}
+
+extern "C" int kvoff_attention_fp8(
+    const void* q, int64_t q_stride_bytes, void* out, int64_t out_stride_bytes, float* lse,
+    const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+    int64_t num_pages, int64_t page_size, int64_t scale_block, const int32_t* block_tables,
+    int64_t table_stride, int64_t table_width, const int32_t* context_lens,
+    const int32_t* cu_seqlens_q, int64_t num_seqs, int64_t num_tokens, int64_t max_seqlen_q,
+    int64_t q_heads, int64_t kv_heads, int64_t head_dim, int32_t dtype, float softmax_scale,
+    void* workspace, int64_t workspace_bytes, void* stream) {
+  if (injected("attention_fp8")) return KVOFF_EINJECTED;
+  if (table_width < 0 || num_pages < 0 || num_pages > 0x7FFFFFFFll || num_tokens < 0 ||
+      q_stride_bytes < 0 || out_stride_bytes < 0 || table_stride < 0 ||
+      (page_size > 0 && table_width > 0x7FFFFF00ll / page_size))
+    return fail(KVOFF_EINVAL, "kvoff_attention_fp8: bad sizes");
+  const attention::Shape s{num_seqs, max_seqlen_q, table_width * page_size, q_heads, kv_heads, head_dim};
+  KVOFF_TRY(attention::check_shape(s, page_size));
+  if (scale_block < 16 || (scale_block & (scale_block - 1)) != 0 || page_size % scale_block != 0)
+    return fail(KVOFF_EINVAL,
+                "kvoff_attention_fp8: a scale block is 16 * 2^n tokens and divides the page of %lld",
+                (long long)page_size);
+  if (dtype != KVOFF_BF16 && dtype != KVOFF_FP16)
+    return fail(KVOFF_EINVAL, "kvoff_attention_fp8: q and out are bf16 or fp16");
+  if (cu_seqlens_q == nullptr && (num_tokens != num_seqs || max_seqlen_q != 1))
+    return fail(KVOFF_EINVAL, "kvoff_attention_fp8: without cu_seqlens_q each sequence has one token");
+  if (num_tokens > 0x7FFFFFFFll / q_heads)
+    return fail(KVOFF_EINVAL, "kvoff_attention_fp8: sizes exceed 32 bits");
+  if (num_seqs == 0 || num_tokens == 0 || max_seqlen_q == 0) return ok();
+  if (q == nullptr || out == nullptr || context_lens == nullptr ||
+      (s.keys > 0 && (k_cache == nullptr || v_cache == nullptr || k_scale == nullptr ||
+                      v_scale == nullptr || block_tables == nullptr)))
+    return fail(KVOFF_EINVAL, "kvoff_attention_fp8: null pointer");
+  const uintptr_t wide = reinterpret_cast<uintptr_t>(q) | (uintptr_t)q_stride_bytes |
+                         reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache);
+  const uintptr_t pairs = reinterpret_cast<uintptr_t>(out) | (uintptr_t)out_stride_bytes;
+  if ((wide & 15u) != 0 || (pairs & 3u) != 0)
+    return fail(KVOFF_EINVAL,
+                "kvoff_attention_fp8: q and the caches must be 16-byte aligned, out 4-byte");
+  const attention::Choice c = attention::choose(s);
+  const int64_t need = attention::workspace_of(c, head_dim);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need ||
+                   (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0))
+    return fail(KVOFF_EINVAL, "kvoff_attention_fp8: needs a 16-byte aligned workspace of %lld bytes",
+                (long long)need);
+  attention::Args a{};
+  a.q = static_cast<const uint8_t*>(q);
+  a.out = static_cast<uint8_t*>(out);
+  a.lse = lse;
+  a.q_stride = q_stride_bytes;
+  a.out_stride = out_stride_bytes;
+  a.cache[0] = static_cast<const uint8_t*>(k_cache);
+  a.cache[1] = static_cast<const uint8_t*>(v_cache);
+  a.scale[0] = k_scale;
+  a.scale[1] = v_scale;
+  a.tables = block_tables;
+  a.table_stride = table_stride;
+  a.contexts = context_lens;
+  a.starts = cu_seqlens_q;
+  a.scale_log2 = softmax_scale * 1.4426950408889634f;
+  a.table_width = (int32_t)table_width;
+  a.num_pages = (int32_t)num_pages;
+  a.page = (int32_t)page_size;
+  a.block_tiles = (int32_t)(scale_block / 16);
+  a.seqs = (int32_t)num_seqs;
+  a.num_tokens = (int32_t)num_tokens;
+  a.q_heads = (int32_t)q_heads;
+  a.kv_heads = (int32_t)kv_heads;
+  a.group = (int32_t)(q_heads / kv_heads);
+  a.rows = c.rows;
+  a.max_tiles = (int32_t)c.max_tiles;
+  a.direct = c.direct;
+  a.bf16 = dtype == KVOFF_BF16;
+  a.records = static_cast<attention::Record*>(workspace);
+  a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
+                                       c.grid * (int64_t)sizeof(attention::Record));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  KVOFF_TRY(attention::launch_decode(a, (int)head_dim, c.grid, st));
+  if (!c.direct) KVOFF_TRY(attention::launch_join(a, (int)head_dim, c.grid, st));
+  return ok();
+}

@@ -1,0 +1,292 @@
+// Shared by the attention kernels over the e4m3 paged cache: arguments, the
+// partition of the work over CTAs, and the join of split rows.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "runtime.h"
+
+namespace kvoff {
+namespace attention {
+
+// Keys of one step of the partition.
+constexpr int kKeyTile = 128;
+
+struct Args {
+  const uint8_t* q;
+  uint8_t* out;
+  float* lse;  // [num_tokens, q_heads] or null
+  int64_t q_stride, out_stride;  // bytes per token
+  const uint8_t* cache[2];       // K, V: [pages, page, kv_heads, D]
+  const float* scale[2];         // [pages, page / scale_block, kv_heads]
+  const int32_t* tables;
+  int64_t table_stride;
+  const int32_t* contexts;
+  const int32_t* starts;  // null: token s is sequence s
+  float scale_log2;       // softmax scale * log2(e)
+  int32_t table_width, num_pages, page, block_tiles;  // scale block in 16-key units
+  int32_t seqs, num_tokens, q_heads, kv_heads, group;
+  int32_t rows;      // packed rows of a row tile
+  int32_t max_tiles; // row tiles of the longest sequence (direct form)
+  bool direct;       // one CTA per (sequence, head, row tile), nothing is split
+  bool bf16;
+  float* partial;            // 2 slots per CTA
+  struct Record* records;    // one per CTA
+};
+
+// What a CTA leaves for the join: the split (sequence, head, row tile) that
+// begins in it, how many CTAs after it hold parts of it, and which of its two
+// slots hold a part. Slot 0 continues the previous CTA's last tile, slot 1
+// begins the CTA's own last one.
+struct Record {
+  int32_t seq, head, tile, further;
+  int32_t valid[2];
+  int32_t pad[2];
+};
+
+// The rows of a sequence and what they see. Row i of a (sequence, KV head) is
+// query token i / group, head i % group; token t of q_len sees keys below
+// context - q_len + t + 1.
+struct Sequence {
+  int32_t start, q_len, context, tiles;
+  int64_t base;  // cost of a row tile: base + its last row's index + 1
+
+  __device__ __forceinline__ void load(const Args& a, int s) {
+    if (a.starts == nullptr) {
+      start = s;
+      q_len = 1;
+    } else {  // kept inside q whatever the offsets say
+      start = min(max(a.starts[s], 0), a.num_tokens);
+      q_len = min(max(a.starts[s + 1], start), a.num_tokens) - start;
+    }
+    const int64_t room = (int64_t)a.table_width * a.page;
+    context = (int32_t)min((int64_t)max(a.contexts[s], 0), room);
+    const int64_t rows = (int64_t)q_len * a.group;
+    tiles = (int32_t)((rows + a.rows - 1) / a.rows);
+    base = (int64_t)max(context - q_len, 0) * a.group;
+  }
+  __device__ __forceinline__ int64_t cost(const Args& a, int r) const {
+    return base + min((int64_t)(r + 1) * a.rows, (int64_t)q_len * a.group);
+  }
+  // Cost of the row tiles before r (all of them whole).
+  __device__ __forceinline__ int64_t before(const Args& a, int64_t r) const {
+    return r * base + a.rows * (r * (r + 1) / 2);
+  }
+  __device__ __forceinline__ int64_t per_head(const Args& a) const {
+    return tiles == 0 ? 0 : before(a, tiles - 1) + cost(a, tiles - 1);
+  }
+  // Keys that the last row of tile r sees.
+  __device__ __forceinline__ int keys(const Args& a, int r) const {
+    const int64_t last = min((int64_t)(r + 1) * a.rows, (int64_t)q_len * a.group) - 1;
+    return max(0, context - q_len + (int)(last / a.group) + 1);
+  }
+};
+
+// One row tile of one head, and the key tiles of it that a CTA works through.
+struct Segment {
+  int seq, head, tile;
+  int begin, end, tiles;  // key tiles
+  bool whole;
+  int slot;  // of the partial result, when not whole
+};
+
+// Deals the work of a launch over its CTAs. The key reads of all (sequence,
+// head, row tile) triples stand on one axis, in that order; each CTA takes an
+// equal stretch of it, cut at key tiles. So a batch of unequal lengths, or one
+// long sequence, keeps all SMs busy to the end, from lengths that only the
+// device knows. A triple that is cut is joined by join_kernel.
+//
+//   Walk walk(args); if walk.next(segment) ... until false; walk.finish().
+template <int kThreads>
+struct Walk {
+  const Args& a;
+  Sequence seq;
+  int s, head, tile, cta;
+  int64_t at, from, to, share;  // axis position of the triple; the CTA's stretch
+  Record record;
+  bool more;
+
+  struct Shared {
+    int64_t warp_sum[kThreads / 32];
+    int64_t position;
+    int32_t seq;
+  };
+
+  __device__ __forceinline__ Walk(const Args& args, Shared* sh) : a(args) {
+    cta = blockIdx.x;
+    record.further = -1;
+    record.valid[0] = record.valid[1] = 0;
+    if (a.direct) {
+      tile = cta % a.max_tiles;
+      head = cta / a.max_tiles % a.kv_heads;
+      s = cta / a.max_tiles / a.kv_heads;
+      seq.load(a, s);
+      more = tile < seq.tiles;
+      return;
+    }
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int per = (a.seqs + kThreads - 1) / kThreads;
+    const int first = min((int)threadIdx.x * per, a.seqs), last = min(first + per, a.seqs);
+    int64_t mine = 0;
+    for (int i = first; i < last; ++i) {
+      seq.load(a, i);
+      mine += a.kv_heads * seq.per_head(a);
+    }
+    int64_t sum = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int64_t other = __shfl_up_sync(0xFFFFFFFFu, sum, d);
+      if (lane >= d) sum += other;
+    }
+    if (lane == 31) sh->warp_sum[warp] = sum;
+    __syncthreads();
+    int64_t total = 0, before = sum - mine;
+#pragma unroll
+    for (int i = 0; i < kThreads / 32; ++i) {
+      if (i < warp) before += sh->warp_sum[i];
+      total += sh->warp_sum[i];
+    }
+    // A stretch of less than two key tiles costs more to join than to read.
+    const int64_t least = (int64_t)2 * kKeyTile * a.group;
+    share = max((total + gridDim.x - 1) / gridDim.x, least);
+    from = cta * share;
+    to = min(from + share, total);
+    more = from < to;
+    if (more && from >= before && from < before + mine) {
+      int64_t position = before;
+      for (int i = first; i < last; ++i) {
+        seq.load(a, i);
+        const int64_t cost = a.kv_heads * seq.per_head(a);
+        if (from < position + cost) {
+          sh->position = position;
+          sh->seq = i;
+          break;
+        }
+        position += cost;
+      }
+    }
+    __syncthreads();
+    if (!more) return;
+    s = sh->seq;
+    at = sh->position;
+    seq.load(a, s);
+    const int64_t per_head = seq.per_head(a);
+    head = (int)((from - at) / per_head);
+    at += head * per_head;
+    int low = 0, high = seq.tiles - 1;  // the last row tile that begins at or before `from`
+    while (low < high) {
+      const int mid = (low + high + 1) / 2;
+      if (at + seq.before(a, mid) <= from)
+        low = mid;
+      else
+        high = mid - 1;
+    }
+    tile = low;
+    at += seq.before(a, tile);
+  }
+
+  // The key tile at which the axis position x cuts the current triple.
+  __device__ __forceinline__ int cut(int64_t x, int64_t cost, int tiles) const {
+    if (x <= at) return 0;
+    if (x >= at + cost) return tiles;
+    return (int)min((int64_t)tiles, (x - at) / ((int64_t)kKeyTile * a.group));
+  }
+
+  __device__ __forceinline__ void advance() {
+    if (a.direct) {  // more row tiles than announced: the same CTAs take them
+      tile += a.max_tiles;
+      more = tile < seq.tiles;
+      return;
+    }
+    at += seq.cost(a, tile);
+    more = at < to;
+    if (!more || ++tile < seq.tiles) return;
+    tile = 0;
+    if (++head < a.kv_heads) return;
+    head = 0;
+    do seq.load(a, ++s);  // `to` is at most the total, so a sequence with rows follows
+    while (seq.tiles == 0);
+  }
+
+  __device__ __forceinline__ bool next(Segment* out) {
+    while (more) {
+      out->seq = s;
+      out->head = head;
+      out->tile = tile;
+      const int keys = seq.keys(a, tile);
+      out->tiles = max(1, (keys + kKeyTile - 1) / kKeyTile);
+      out->begin = 0;
+      out->end = out->tiles;
+      out->slot = 0;
+      if (!a.direct) {
+        const int64_t cost = seq.cost(a, tile);
+        out->begin = cut(from, cost, out->tiles);
+        out->end = cut(to, cost, out->tiles);
+        out->slot = at >= from ? 1 : 0;
+        out->whole = out->begin == 0 && out->end == out->tiles;
+        const bool part = !out->whole && out->begin < out->end;
+        if (part && out->slot == 0) record.valid[0] = 1;
+        if (part && out->slot == 1) record.valid[1] = 1;
+        if (out->slot == 1 && !out->whole) {
+          record.seq = s;
+          record.head = head;
+          record.tile = tile;
+          record.further = (int32_t)((at + cost - 1) / share) - cta;
+        }
+      } else {
+        out->whole = true;
+      }
+      if (out->begin < out->end) return true;
+      advance();
+    }
+    return false;
+  }
+
+  __device__ __forceinline__ void finish() {
+    if (!a.direct && threadIdx.x == 0) a.records[cta] = record;
+  }
+};
+
+// A slot of the partial results: sums of p * v [rows, D], then each row's
+// maximum (log2 units) and its sum of p.
+__host__ __device__ inline int64_t slot_floats(int rows, int dim) {
+  return (int64_t)rows * (dim + 2);
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Writes two adjacent output values of a row.
+__device__ __forceinline__ void write_pair(const Args& a, int token, int q_head, int dim, int d,
+                                           float x, float y) {
+  uint8_t* p = a.out + token * a.out_stride + ((int64_t)q_head * dim + d) * 2;
+  if (a.bf16)
+    *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(x, y);
+  else
+    *reinterpret_cast<__half2*>(p) = __floats2half2_rn(x, y);
+}
+
+__device__ __forceinline__ void write_lse(const Args& a, int token, int q_head, float m, float l) {
+  // l == 0: the row sees no key.
+  if (a.lse != nullptr)
+    a.lse[(int64_t)token * a.q_heads + q_head] =
+        l == 0.0f ? __int_as_float(0xFF800000) : (m + log2f(l)) * 0.69314718055994531f;
+}
+
+// Joins the split row tiles; one CTA of `grid` per record and 32 values of D.
+int launch_join(const Args& a, int dim, int grid, cudaStream_t stream);
+
+// The kernels. `dim` is 64 or 128; a is filled but for rows and partial.
+constexpr int kDecodeRows = 16;
+int decode_grid();
+int decode_rows(int64_t rows);  // rows of a row tile for `rows` packed rows a head
+int launch_decode(const Args& a, int dim, int grid, cudaStream_t stream);
+
+}  // namespace attention
+}  // namespace kvoff

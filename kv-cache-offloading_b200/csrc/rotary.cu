@@ -1,0 +1,260 @@
+// Rotary positions of q and k.
+//
+// A head's first R = rotary_dim values are R/2 pairs; pair j of a token at
+// position p is turned by the angle p * f_j, whose cosine and sine (with the
+// attention factor of a scaled rotation already in them) stand in row p of a
+// table [positions, R]: cosines first, then sines.
+//     y1 = x1 * c - x2 * s,   y2 = x2 * c + x1 * s
+// Pair j is (x_j, x_{j + R/2}) in the half layout and (x_2j, x_2j+1) in the
+// interleaved one; values from R on pass through. The transpose of the map
+// (s -> -s) is its gradient. Products and sums are fp32, one rounding at the
+// end.
+//
+// Bound by memory: each value is read and written once, and a table row is
+// read once per token. A thread owns one unit of a token (the half layout: a
+// 16-byte vector of the first half with its partner in the second; the
+// interleaved one: a 16-byte vector, which holds whole pairs) and carries its
+// cosines and sines in registers through several heads. With all heads of a
+// unit in one thread a decode step of four tokens would use a few warps only,
+// and with one head per thread every thread would load more table than data,
+// so the heads are dealt over `lanes` threads: one head each while the grid
+// is small, four once the tokens alone fill the GPU.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "runtime.h"
+
+namespace kvoff {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kUnroll = 4;  // heads whose loads are in flight at once
+
+struct RotaryArgs {
+  const uint8_t* in[2];  // q, k
+  uint8_t* out[2];
+  int64_t in_stride[2], out_stride[2];  // bytes per token
+  const void* positions;
+  const float* table;
+  int64_t table_rows, num_tokens;
+  int32_t* bad_positions;
+  int32_t heads[2];
+  int32_t dim, rotary_dim;
+  int32_t units, turning;  // units of a head; the first `turning` hold pairs
+  int32_t lanes, tokens_per_cta;
+  float sign;       // of the sines: -1 for the transpose
+  bool positions64, copy;  // copy: units that pass through are written too
+};
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T x);
+template <>
+__device__ __forceinline__ float to_f32(float x) { return x; }
+template <>
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <>
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ __half from_f32(float x) { return __float2half_rn(x); }
+
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Vec {
+  T x[V];
+};
+
+// V values per vector; a unit is two vectors in the half layout, one else.
+template <typename T, int V, bool kInterleaved>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
+  constexpr int kPairs = kInterleaved ? V / 2 : V;
+  using Vector = Vec<T, V>;
+  const int per_token = a.units * a.lanes;
+  const int64_t token = (int64_t)blockIdx.x * a.tokens_per_cta + threadIdx.x / per_token;
+  const int rest = threadIdx.x % per_token;
+  const int unit = rest % a.units, lane = rest / a.units;
+  if (threadIdx.x >= a.tokens_per_cta * per_token || token >= a.num_tokens) return;
+  const int64_t position = a.positions64 ? static_cast<const int64_t*>(a.positions)[token]
+                                         : static_cast<const int32_t*>(a.positions)[token];
+  if (position < 0) return;
+  if (position >= a.table_rows) {
+    if (rest == 0 && a.bad_positions != nullptr) atomicAdd(a.bad_positions, 1);
+    return;
+  }
+  const bool turns = unit < a.turning;
+  if (!turns && !a.copy) return;
+  const int half = a.rotary_dim / 2;
+  // First value of the unit, and of its partner vector.
+  const int at = turns ? unit * V : a.rotary_dim + (unit - a.turning) * V;
+  const int partner = (!kInterleaved && turns) ? at + half : at;
+  float c[kPairs], s[kPairs];
+  if (turns) {
+    const float* row = a.table + position * a.rotary_dim + unit * kPairs;
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      c[i] = __ldg(row + i);
+      s[i] = a.sign * __ldg(row + half + i);
+    }
+  }
+  const int heads = a.heads[0] + a.heads[1];
+  for (int first = lane; first < heads; first += kUnroll * a.lanes) {
+    Vector x[kUnroll], y[kUnroll];
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      const int h = first + i * a.lanes;
+      if (h < heads) {
+        const bool is_k = h >= a.heads[0];
+        const uint8_t* p = (is_k ? a.in[1] + token * a.in_stride[1] : a.in[0] + token * a.in_stride[0]) +
+                           (int64_t)(is_k ? h - a.heads[0] : h) * a.dim * sizeof(T);
+        x[i] = *reinterpret_cast<const Vector*>(p + at * sizeof(T));
+        if (!kInterleaved) y[i] = *reinterpret_cast<const Vector*>(p + partner * sizeof(T));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      const int h = first + i * a.lanes;
+      if (h < heads) {
+        const bool is_k = h >= a.heads[0];
+        uint8_t* p = (is_k ? a.out[1] + token * a.out_stride[1] : a.out[0] + token * a.out_stride[0]) +
+                     (int64_t)(is_k ? h - a.heads[0] : h) * a.dim * sizeof(T);
+        if (turns) {
+#pragma unroll
+          for (int j = 0; j < kPairs; ++j) {
+            T& first_of = kInterleaved ? x[i].x[2 * j] : x[i].x[j];
+            T& second_of = kInterleaved ? x[i].x[2 * j + 1] : y[i].x[j];
+            const float x1 = to_f32(first_of), x2 = to_f32(second_of);
+            first_of = from_f32<T>(x1 * c[j] - x2 * s[j]);
+            second_of = from_f32<T>(x2 * c[j] + x1 * s[j]);
+          }
+          if (!kInterleaved) *reinterpret_cast<Vector*>(p + partner * sizeof(T)) = y[i];
+        }
+        *reinterpret_cast<Vector*>(p + at * sizeof(T)) = x[i];
+      }
+    }
+  }
+}
+
+template <typename T, int V, bool kInterleaved>
+int launch(RotaryArgs a, cudaStream_t stream) {
+  a.turning = a.rotary_dim / (kInterleaved ? V : 2 * V);
+  a.units = a.turning + (a.copy ? (a.dim - a.rotary_dim) / V : 0);
+  const int heads = a.heads[0] + a.heads[1];
+  if (a.units > kThreads)
+    return fail(KVOFF_EINVAL, "kvoff_rotary: heads of %d values at this alignment are not supported",
+                a.dim);
+  // Four heads a thread once one thread per (token, unit, 4 heads) fills the
+  // GPU; below that, as many lanes as the block has room for.
+  const int64_t full = (int64_t)sm_count() * 2048;
+  int lanes = (heads + kUnroll - 1) / kUnroll;
+  if (a.num_tokens * a.units * lanes < full) lanes = heads;
+  const int most = kThreads / a.units;
+  a.lanes = lanes < most ? lanes : most;
+  const int per_token = a.units * a.lanes;
+  a.tokens_per_cta = a.num_tokens * per_token < full ? 1 : kThreads / per_token;
+  const int threads = (a.tokens_per_cta * per_token + 31) / 32 * 32;
+  const int64_t grid = (a.num_tokens + a.tokens_per_cta - 1) / a.tokens_per_cta;
+  rotary_kernel<T, V, kInterleaved><<<(unsigned)grid, threads, 0, stream>>>(a);
+  return cuda_status(cudaGetLastError(), "rotary launch");
+}
+
+template <typename T>
+int launch_layout(const RotaryArgs& a, bool interleaved, uintptr_t bits, cudaStream_t stream) {
+  constexpr int V = 16 / sizeof(T);
+  // The vector forms need every address and stride in whole vectors, and a
+  // rotated part (per half, in the half layout) of whole vectors.
+  const bool wide = (bits & 15u) == 0 && a.dim % V == 0;
+  if (interleaved)
+    return wide && a.rotary_dim % V == 0 ? launch<T, V, true>(a, stream)
+                                         : launch<T, 2, true>(a, stream);
+  return wide && a.rotary_dim % (2 * V) == 0 ? launch<T, V, false>(a, stream)
+                                             : launch<T, 1, false>(a, stream);
+}
+
+}  // namespace
+}  // namespace kvoff
+
+using namespace kvoff;
+
+extern "C" int kvoff_rotary(const void* q, int64_t q_stride_bytes, void* q_out,
+                            int64_t q_out_stride_bytes, int64_t q_heads, const void* k,
+                            int64_t k_stride_bytes, void* k_out, int64_t k_out_stride_bytes,
+                            int64_t kv_heads, int64_t head_dim, int64_t rotary_dim, int32_t dtype,
+                            const void* positions, int32_t position_bytes, const float* table,
+                            int64_t table_rows, int64_t num_tokens, int32_t flags,
+                            int32_t* bad_positions, void* stream) {
+  if (injected("rotary")) return KVOFF_EINJECTED;
+  if (num_tokens < 0 || q_heads < 0 || kv_heads < 0 || q_heads + kv_heads <= 0 || head_dim <= 0 ||
+      table_rows < 0 || q_stride_bytes < 0 || q_out_stride_bytes < 0 || k_stride_bytes < 0 ||
+      k_out_stride_bytes < 0 || q_heads + kv_heads > 65535 || head_dim > 65535)
+    return fail(KVOFF_EINVAL, "kvoff_rotary: bad sizes");
+  if (rotary_dim <= 0 || rotary_dim % 2 != 0 || rotary_dim > head_dim)
+    return fail(KVOFF_EINVAL, "kvoff_rotary: rotary_dim %lld must be even and at most head_dim %lld",
+                (long long)rotary_dim, (long long)head_dim);
+  if (dtype != KVOFF_BF16 && dtype != KVOFF_FP16 && dtype != KVOFF_FP32)
+    return fail(KVOFF_EINVAL, "kvoff_rotary: unknown dtype %d", (int)dtype);
+  if (position_bytes != 4 && position_bytes != 8)
+    return fail(KVOFF_EINVAL, "kvoff_rotary: positions are int32 or int64");
+  if ((flags & ~(KVOFF_ROTARY_INTERLEAVED | KVOFF_ROTARY_INVERSE)) != 0)
+    return fail(KVOFF_EINVAL, "kvoff_rotary: unknown flags %d", (int)flags);
+  if (num_tokens == 0) return ok();
+  if (num_tokens > 0x7FFFFFFFll)
+    return fail(KVOFF_EINVAL, "kvoff_rotary: %lld tokens exceed one launch",
+                (long long)num_tokens);
+  if ((q_heads > 0 && (q == nullptr || q_out == nullptr)) ||
+      (kv_heads > 0 && (k == nullptr || k_out == nullptr)) || positions == nullptr ||
+      table == nullptr)
+    return fail(KVOFF_EINVAL, "kvoff_rotary: null pointer");
+  const bool interleaved = (flags & KVOFF_ROTARY_INTERLEAVED) != 0;
+  const int elem = dtype == KVOFF_FP32 ? 4 : 2;
+  uintptr_t bits = 0;
+  if (q_heads > 0)
+    bits |= reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(q_out) |
+            (uintptr_t)q_stride_bytes | (uintptr_t)q_out_stride_bytes;
+  if (kv_heads > 0)
+    bits |= reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(k_out) |
+            (uintptr_t)k_stride_bytes | (uintptr_t)k_out_stride_bytes;
+  // The narrow interleaved form moves one pair at a time.
+  const int narrow = interleaved ? 2 * elem : elem;
+  if (bits % narrow != 0 || (interleaved && head_dim % 2 != 0))
+    return fail(KVOFF_EINVAL, "kvoff_rotary: rows must be aligned to %d bytes%s", narrow,
+                interleaved ? " and hold an even number of values" : "");
+  RotaryArgs a{};
+  a.in[0] = static_cast<const uint8_t*>(q);
+  a.in[1] = static_cast<const uint8_t*>(k);
+  a.out[0] = static_cast<uint8_t*>(q_out);
+  a.out[1] = static_cast<uint8_t*>(k_out);
+  a.in_stride[0] = q_stride_bytes;
+  a.in_stride[1] = k_stride_bytes;
+  a.out_stride[0] = q_out_stride_bytes;
+  a.out_stride[1] = k_out_stride_bytes;
+  a.positions = positions;
+  a.positions64 = position_bytes == 8;
+  a.table = table;
+  a.table_rows = table_rows;
+  a.num_tokens = num_tokens;
+  a.bad_positions = bad_positions;
+  a.heads[0] = (int32_t)q_heads;
+  a.heads[1] = (int32_t)kv_heads;
+  a.dim = (int32_t)head_dim;
+  a.rotary_dim = (int32_t)rotary_dim;
+  a.sign = (flags & KVOFF_ROTARY_INVERSE) != 0 ? -1.0f : 1.0f;
+  a.copy = rotary_dim < head_dim &&
+           ((q_heads > 0 && q != q_out) || (kv_heads > 0 && k != k_out));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int rc;
+  if (dtype == KVOFF_BF16)
+    rc = launch_layout<__nv_bfloat16>(a, interleaved, bits, s);
+  else if (dtype == KVOFF_FP16)
+    rc = launch_layout<__half>(a, interleaved, bits, s);
+  else
+    rc = launch_layout<float>(a, interleaved, bits, s);
+  if (rc != KVOFF_OK) return rc;
+  return ok();
+}

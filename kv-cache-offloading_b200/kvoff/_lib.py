@@ -17,6 +17,8 @@ ABI_VERSION = 1
 KVOFF_OK, KVOFF_EINVAL, KVOFF_ECUDA, KVOFF_EINJECTED, KVOFF_ENOMEM, KVOFF_EDEVICE = range(6)
 SAVE, RESTORE = 0, 1
 COPY_ENGINE, COPY_TMA, COPY_SM = 0, 1, 2
+BF16, FP16, FP32 = 0, 1, 2
+ROTARY_INTERLEAVED, ROTARY_INVERSE = 1, 2
 
 _P = ctypes.c_void_p
 _PP = ctypes.POINTER(ctypes.c_void_p)
@@ -56,6 +58,15 @@ SIGNATURES = {
                                          _I32, _P]),
     "kvoff_store_kvcache": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _P, _I64, _P, _I64, _I64, _P,
                                            _P]),
+    "kvoff_rotary": (ctypes.c_int, [_P, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64,
+                                    _I32, _P, _I32, _P, _I64, _I64, _I32, _P, _P]),
+    "kvoff_store_kvcache_fp8": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I32,
+                                               _I64, _P, _I64, _I64, _P, _P]),
+    "kvoff_attention_fp8": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _P, _P, _P, _P, _I64, _I64, _I64,
+                                           _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64,
+                                           _I64, _I32, ctypes.c_float, _P, _I64, _P]),
+    "kvoff_attention_fp8_workspace": (ctypes.c_int, [_I64, _I64, _I64, _I64, _I64, _I64, _I64,
+                                                     _PI64]),
     "kvoff_host_alloc": (ctypes.c_int, [ctypes.c_uint64, _I32, _PP, _PP]),
     "kvoff_host_free": (ctypes.c_int, [_P]),
     "kvoff_device_numa_node": (ctypes.c_int, [_I32, ctypes.POINTER(_I32)]),

@@ -9,6 +9,7 @@ pointers so that one call can target pinned host slabs, their device aliases
 from __future__ import annotations
 
 import ctypes
+import math
 from dataclasses import dataclass
 
 import torch
@@ -392,3 +393,332 @@ def _store_fn():
     if _STORE is None:
         _STORE = _lib.lib().kvoff_store_kvcache
     return _STORE
+
+
+# ---------------------------------------------------------------------------
+# Rotary positions, the e4m3 paged cache and attention over it
+#
+# A layer's three calls, in order: rotary(q, k), store_kvcache_fp8(k, v) and
+# attention_fp8(q). Like store_kvcache they run once per layer per forward, so
+# their host paths are kept short.
+
+_DTYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16, torch.float32: _lib.FP32}
+_FP8 = torch.float8_e4m3fn
+
+
+def _launch(name: str, args: tuple, device: torch.device, stream) -> None:
+    """Call entry point `name` on `device` and raise KvoffError on a failure."""
+    if device.index == torch.cuda.current_device():
+        status = _entry(name)(*args, _fast_stream(device, stream))
+    else:
+        with torch.cuda.device(device):
+            status = _entry(name)(*args, _fast_stream(device, stream))
+    if status:
+        _lib.check(status, name)
+
+
+_ENTRIES: dict = {}
+
+
+def _entry(name: str):
+    fn = _ENTRIES.get(name)
+    if fn is None:
+        fn = _ENTRIES[name] = getattr(_lib.lib(), name)
+    return fn
+
+
+def _same_device(device: torch.device, *tensors) -> None:
+    if device.type != "cuda":
+        raise ValueError("the tensors must be CUDA tensors")
+    for t in tensors:
+        if t.device != device:
+            raise ValueError("the tensors must be on one CUDA device")
+
+
+def _rows(x: torch.Tensor, what: str) -> int:
+    """Bytes from one token to the next of x [N, H, D] with dense heads."""
+    if x.dim() != 3:
+        raise ValueError(f"{what} must be [tokens, heads, head_dim]")
+    stride, shape = x.stride(), x.shape
+    if (stride[2] != 1 and shape[2] > 1) or (stride[1] != shape[2] and shape[1] > 1):
+        raise ValueError(f"the heads of {what} must be dense")
+    return stride[0] * x.element_size()
+
+
+def rotary_table(positions: int, rotary_dim: int, *, base: float = 10000.0,
+                 scaling: dict | None = None, device=None) -> torch.Tensor:
+    """Cosines and sines of the first `positions` positions, for `rotary`.
+
+    Returns fp32 [positions, rotary_dim]: row p holds cos(p * f_j), then
+    sin(p * f_j), of the rotary_dim / 2 pairs, f_j = base^(-2j / rotary_dim).
+    Angles are formed in 64 bits. `scaling` stretches the frequencies for
+    contexts longer than the model was trained on; its "type" is one of
+
+    * "linear": f_j / factor;
+    * "ntk": the base grows to base * factor^(R / (R - 2)), R = rotary_dim;
+    * "yarn": f_j / factor for pairs that turn less than beta_slow (1) times
+      over original_max_position_embeddings, f_j for those that turn more than
+      beta_fast (32) times, a linear ramp over the pair index between; cosines
+      and sines carry attention_factor (0.1 ln(factor) + 1);
+    * "llama3": f_j / factor for pairs that turn less than low_freq_factor (1)
+      times over original_max_position_embeddings, f_j for those that turn more
+      than high_freq_factor (4) times, a linear blend over the turns between.
+    """
+    if rotary_dim <= 0 or rotary_dim % 2 or positions < 0:
+        raise ValueError("rotary_dim must be even and positive, positions not negative")
+    half = rotary_dim // 2
+    scaling = dict(scaling or {})
+    kind = scaling.pop("type", scaling.pop("rope_type", "none"))
+    known = {"none": (), "linear": ("factor",), "ntk": ("factor",),
+             "yarn": ("factor", "original_max_position_embeddings", "beta_fast", "beta_slow",
+                      "attention_factor"),
+             "llama3": ("factor", "original_max_position_embeddings", "low_freq_factor",
+                        "high_freq_factor")}
+    if kind not in known:
+        raise ValueError(f"unknown rotary scaling {kind!r}")
+    unknown = set(scaling) - set(known[kind])
+    if unknown:
+        raise ValueError(f"rotary scaling {kind!r} does not know {sorted(unknown)}")
+    if kind != "none" and not float(scaling.get("factor", 0.0)) >= 1.0:
+        raise ValueError(f"rotary scaling {kind!r} needs a factor of 1 or more")
+    if kind in ("yarn", "llama3") and not scaling.get("original_max_position_embeddings", 0) > 0:
+        raise ValueError(f"rotary scaling {kind!r} needs original_max_position_embeddings")
+    factor = float(scaling.get("factor", 1.0))
+    original = float(scaling.get("original_max_position_embeddings", 0))
+    if kind == "ntk":
+        base = base * factor ** (rotary_dim / max(1, rotary_dim - 2))
+    freq = float(base) ** (-torch.arange(half, dtype=torch.float64) / half)
+    attention = 1.0
+    if kind == "linear":
+        freq = freq / factor
+    elif kind == "yarn":
+        def pair_that_turns(times: float) -> float:
+            return half * math.log(original / (times * 2 * math.pi)) / math.log(base)
+
+        low = max(math.floor(pair_that_turns(float(scaling.get("beta_fast", 32.0)))), 0)
+        high = min(math.ceil(pair_that_turns(float(scaling.get("beta_slow", 1.0)))), rotary_dim - 1)
+        ramp = ((torch.arange(half, dtype=torch.float64) - low) / max(high - low, 0.001)).clamp(0, 1)
+        freq = freq / factor * ramp + freq * (1 - ramp)
+        attention = float(scaling.get("attention_factor", 0.1 * math.log(factor) + 1.0))
+    elif kind == "llama3":
+        low = float(scaling.get("low_freq_factor", 1.0))
+        high = float(scaling.get("high_freq_factor", 4.0))
+        if not high > low:
+            raise ValueError("high_freq_factor must be above low_freq_factor")
+        blend = ((original * freq / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
+        freq = (1 - blend) * freq / factor + blend * freq
+    angle = torch.outer(torch.arange(positions, dtype=torch.float64, device=device), freq.to(device))
+    return torch.cat([angle.cos() * attention, angle.sin() * attention], dim=1).float()
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, *,
+           interleaved: bool = False, inverse: bool = False, out=None,
+           bad_positions: torch.Tensor | None = None, stream=None):
+    """Turn q [N, Hq, D] and k [N, Hk, D] to their positions; returns (q, k).
+
+    `table` [P, R] comes from `rotary_table`; positions are int64 or int32
+    [N]. Pairs are (x_j, x_{j + R/2}), or (x_2j, x_2j+1) when `interleaved`;
+    values from R on pass through. In place unless out=(q_out, k_out) is given
+    (tensors that do not overlap q and k). `inverse` applies the transposed map:
+    the gradient of q and k from that of the result. A negative position
+    leaves its token's rows unwritten, as -1 does in store_kvcache; so does one
+    behind the table, which `bad_positions` (int32, CUDA) counts.
+    """
+    q_out, k_out = (q, k) if out is None else out
+    n, q_heads, dim = q.shape
+    n_k, kv_heads, dim_k = k.shape
+    if n_k != n or dim_k != dim:
+        raise ValueError("q and k must have the same tokens and head_dim")
+    dtype = q.dtype
+    if dtype not in _DTYPES or k.dtype != dtype or q_out.dtype != dtype or k_out.dtype != dtype:
+        raise ValueError("q, k and the outputs must share a dtype: bf16, fp16 or fp32")
+    if q_out.shape != q.shape or k_out.shape != k.shape:
+        raise ValueError("the outputs must have the shapes of q and k")
+    if positions.dtype not in (torch.int64, torch.int32) or positions.shape != (n,) \
+            or not positions.is_contiguous():
+        raise ValueError("positions must be contiguous int64 or int32, one for each token")
+    if table.dtype != torch.float32 or table.dim() != 2 or not table.is_contiguous():
+        raise ValueError("table must be contiguous fp32 [positions, rotary_dim]")
+    device = q.device
+    _same_device(device, k, q_out, k_out, positions, table)
+    if bad_positions is not None:
+        if bad_positions.dtype != torch.int32:
+            raise ValueError("bad_positions must be int32")
+        _same_device(device, bad_positions)
+    flags = (_lib.ROTARY_INTERLEAVED if interleaved else 0) | (_lib.ROTARY_INVERSE if inverse else 0)
+    _launch("kvoff_rotary",
+            (q.data_ptr(), _rows(q, "q"), q_out.data_ptr(), _rows(q_out, "q_out"), q_heads,
+             k.data_ptr(), _rows(k, "k"), k_out.data_ptr(), _rows(k_out, "k_out"), kv_heads, dim,
+             table.shape[1], _DTYPES[dtype], positions.data_ptr(), positions.element_size(),
+             table.data_ptr(), table.shape[0], n, flags,
+             bad_positions.data_ptr() if bad_positions is not None else None), device, stream)
+    return q_out, k_out
+
+
+def _fp8_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+               v_scale: torch.Tensor) -> int:
+    """Check an e4m3 cache [pages, page, H, D] and its scales; tokens of a scale block."""
+    shape, scales = k_cache.shape, k_scale.shape
+    if len(shape) != 4 or v_cache.shape != shape:
+        raise ValueError("k_cache and v_cache must be [pages, page, heads, head_dim], alike")
+    if k_cache.dtype != _FP8 or v_cache.dtype != _FP8:
+        raise ValueError("the caches must be float8_e4m3fn")
+    if len(scales) != 3 or v_scale.shape != scales or scales[0] != shape[0] or scales[2] != shape[2] \
+            or scales[1] <= 0 or shape[1] % scales[1]:
+        raise ValueError("the scales must be [pages, page / scale_block, heads]")
+    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+        raise ValueError("the scales must be fp32")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous()
+            and v_scale.is_contiguous()):
+        raise ValueError("caches and scales must be contiguous")
+    return shape[1] // scales[1]
+
+
+def store_kvcache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
+                      v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                      slot_mapping: torch.Tensor, *, bad_slots: torch.Tensor | None = None,
+                      stream=None) -> None:
+    """Quantize row i of key/value [N, H, D] into e4m3 cache slot slot_mapping[i] (-1: skip).
+
+    Caches are float8_e4m3fn [pages, page, H, D], scales fp32 [pages, page /
+    scale_block, H]: one power of two for each block of scale_block tokens and
+    head. A call that writes a block's first token opens the block; later calls
+    that need a larger scale rescale the rows that are there (see
+    include/kvoff.h). Allocate the scales zeroed. One CUDA-graph-capturable
+    launch, at most 65536 tokens.
+    """
+    num_tokens, heads, dim = key.shape
+    if value.shape != key.shape:
+        raise ValueError("key and value shapes differ")
+    dtype = key.dtype
+    if dtype not in (torch.bfloat16, torch.float16) or value.dtype != dtype:
+        raise ValueError("key and value must both be bf16 or fp16")
+    block = _fp8_cache(k_cache, v_cache, k_scale, v_scale)
+    shape = k_cache.shape
+    if shape[2] != heads or shape[3] != dim:
+        raise ValueError("cache slots must hold [H, D] rows")
+    if slot_mapping.dtype != torch.int32 or slot_mapping.numel() != num_tokens \
+            or not slot_mapping.is_contiguous():
+        raise ValueError("slot_mapping must be contiguous int32, one slot per token")
+    device = key.device
+    _same_device(device, value, k_cache, v_cache, k_scale, v_scale, slot_mapping)
+    if bad_slots is not None:
+        if bad_slots.dtype != torch.int32:
+            raise ValueError("bad_slots must be int32")
+        _same_device(device, bad_slots)
+    _launch("kvoff_store_kvcache_fp8",
+            (key.data_ptr(), _rows(key, "key"), value.data_ptr(), _rows(value, "value"),
+             k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), heads,
+             dim, _DTYPES[dtype], block, slot_mapping.data_ptr(), num_tokens, shape[0] * shape[1],
+             bad_slots.data_ptr() if bad_slots is not None else None), device, stream)
+
+
+_WORKSPACE_BYTES: dict = {}
+
+
+def attention_fp8_workspace(num_seqs: int, max_seqlen_q: int, table_width: int, page_size: int,
+                            q_heads: int, kv_heads: int, head_dim: int, *, device=None) -> int:
+    """Workspace bytes that an attention_fp8 call of these sizes needs on `device`."""
+    index = torch.device(device).index if device is not None else None
+    if index is None:
+        index = torch.cuda.current_device()
+    sizes = (num_seqs, max_seqlen_q, table_width, page_size, q_heads, kv_heads, head_dim)
+    found = _WORKSPACE_BYTES.get((index, sizes))
+    if found is None:
+        answer = ctypes.c_int64(0)
+        with torch.cuda.device(index):
+            _lib.call("kvoff_attention_fp8_workspace", *sizes, ctypes.byref(answer))
+        if len(_WORKSPACE_BYTES) >= 4096:  # sizes only; a program meets a handful
+            _WORKSPACE_BYTES.clear()
+        found = _WORKSPACE_BYTES[(index, sizes)] = answer.value
+    return found
+
+
+def _empty_on(stream, device: torch.device, make):
+    """make() with memory that belongs to `stream` (None: the current stream)."""
+    if stream is None:
+        return make()
+    if not isinstance(stream, torch.cuda.Stream):
+        stream = torch.cuda.ExternalStream(_stream(device, stream), device=device)
+    with torch.cuda.stream(stream):
+        return make()
+
+
+def attention_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                  k_scale: torch.Tensor, v_scale: torch.Tensor, block_tables: torch.Tensor,
+                  context_lens: torch.Tensor, *, cu_seqlens_q: torch.Tensor | None = None,
+                  max_seqlen_q: int = 1, softmax_scale: float | None = None,
+                  out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
+                  workspace: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """Causal attention of q [N, Hq, D] over an e4m3 paged cache; returns out [N, Hq, D].
+
+    The cache and its scales are store_kvcache_fp8's. Sequence s has its
+    context_lens[s] keys (int32, new tokens included) in the pages that row s
+    of block_tables (int32 [B, width]) names. Without cu_seqlens_q token s is
+    sequence s (a decode step, N == B); with it (int32 [B + 1]) sequence s has
+    the tokens cu_seqlens_q[s] .. cu_seqlens_q[s + 1] - 1, at most
+    max_seqlen_q, the last of them at its context's end. A row that sees no key
+    is zero. softmax_scale defaults to D^-0.5; lse (fp32 [N, Hq]) receives the
+    rows' log-sum-exp. See include/kvoff.h for bad pages and padded rows.
+
+    `out` and `workspace` (uint8, attention_fp8_workspace bytes) are allocated
+    on the call's stream when not given; calls that may overlap need workspaces
+    of their own. Enqueues at most two kernels, copies nothing to the host.
+    """
+    n, q_heads, dim = q.shape
+    block = _fp8_cache(k_cache, v_cache, k_scale, v_scale)
+    pages, page, kv_heads, cache_dim = k_cache.shape
+    if cache_dim != dim:
+        raise ValueError("q and the caches must have the same head_dim")
+    dtype = q.dtype
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("q must be bf16 or fp16")
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 \
+            or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
+        raise ValueError("block_tables must be int32 [sequences, pages] with dense rows")
+    seqs, width = block_tables.shape
+    if context_lens.dtype != torch.int32 or context_lens.shape != (seqs,) \
+            or not context_lens.is_contiguous():
+        raise ValueError("context_lens must be contiguous int32, one for each row of block_tables")
+    device = q.device
+    _same_device(device, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens)
+    starts = None
+    if cu_seqlens_q is not None:
+        if cu_seqlens_q.dtype != torch.int32 or cu_seqlens_q.shape != (seqs + 1,) \
+                or not cu_seqlens_q.is_contiguous():
+            raise ValueError("cu_seqlens_q must be contiguous int32 with one entry more than sequences")
+        _same_device(device, cu_seqlens_q)
+        starts = cu_seqlens_q.data_ptr()
+    elif n != seqs or max_seqlen_q != 1:
+        raise ValueError("without cu_seqlens_q each sequence has one token")
+    if out is None:
+        out = _empty_on(stream, device, lambda: torch.empty((n, q_heads, dim), dtype=dtype, device=device))
+    else:
+        if out.shape != q.shape or out.dtype != dtype:
+            raise ValueError("out must have the shape and dtype of q")
+        _same_device(device, out)
+    if lse is not None:
+        if lse.dtype != torch.float32 or lse.shape != (n, q_heads) or not lse.is_contiguous():
+            raise ValueError("lse must be contiguous fp32 [tokens, q_heads]")
+        _same_device(device, lse)
+    need = attention_fp8_workspace(seqs, max_seqlen_q, width, page, q_heads, kv_heads, dim,
+                                   device=device)
+    if workspace is None:
+        if need:
+            workspace = _empty_on(stream, device,
+                                  lambda: torch.empty(need, dtype=torch.uint8, device=device))
+        have = need
+    else:
+        if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous uint8")
+        _same_device(device, workspace)
+        have = workspace.numel()
+    _launch("kvoff_attention_fp8",
+            (q.data_ptr(), _rows(q, "q"), out.data_ptr(), _rows(out, "out"),
+             lse.data_ptr() if lse is not None else None, k_cache.data_ptr(), v_cache.data_ptr(),
+             k_scale.data_ptr(), v_scale.data_ptr(), pages, page, block, block_tables.data_ptr(),
+             block_tables.stride(0), width, context_lens.data_ptr(), starts, seqs, n, max_seqlen_q,
+             q_heads, kv_heads, dim, _DTYPES[dtype],
+             dim ** -0.5 if softmax_scale is None else softmax_scale,
+             workspace.data_ptr() if workspace is not None else None, have), device, stream)
+    return out
