@@ -14,6 +14,10 @@ namespace attention {
 
 // Keys of one step of the partition.
 constexpr int kKeyTile = 128;
+// What beginning and ending a row tile costs, as keys read: 4.3 us, against
+// 0.5 us a tile of 128 keys. Without it a CTA that gets a hundred short
+// sequences ends last (64 sequences of 0 to 8192 keys: 243 us against 49).
+constexpr int kFixed = 768;
 
 struct Args {
   const uint8_t* q;
@@ -66,7 +70,7 @@ struct Sequence {
     context = (int32_t)min((int64_t)max(a.contexts[s], 0), room);
     const int64_t rows = (int64_t)q_len * a.group;
     tiles = (int32_t)((rows + a.rows - 1) / a.rows);
-    base = (int64_t)max(context - q_len, 0) * a.group;
+    base = (int64_t)(max(context - q_len, 0) + kFixed) * a.group;
   }
   __device__ __forceinline__ int64_t cost(const Args& a, int r) const {
     return base + min((int64_t)(r + 1) * a.rows, (int64_t)q_len * a.group);
@@ -94,7 +98,7 @@ struct Segment {
 };
 
 // Deals the work of a launch over its CTAs. The key reads of all (sequence,
-// head, row tile) triples stand on one axis, in that order; each CTA takes an
+// head, row tile) triples, and a fixed cost of each, stand on one axis, in that order; each CTA takes an
 // equal stretch of it, cut at key tiles. So a batch of unequal lengths, or one
 // long sequence, keeps all SMs busy to the end, from lengths that only the
 // device knows. A triple that is cut is joined by join_kernel.
@@ -150,7 +154,7 @@ struct Walk {
       total += sh->warp_sum[i];
     }
     // A stretch of less than two key tiles costs more to join than to read.
-    const int64_t least = (int64_t)2 * kKeyTile * a.group;
+    const int64_t least = (int64_t)(2 * kKeyTile + kFixed) * a.group;
     share = max((total + gridDim.x - 1) / gridDim.x, least);
     from = cta * share;
     to = min(from + share, total);
@@ -190,9 +194,9 @@ struct Walk {
 
   // The key tile at which the axis position x cuts the current triple.
   __device__ __forceinline__ int cut(int64_t x, int64_t cost, int tiles) const {
-    if (x <= at) return 0;
     if (x >= at + cost) return tiles;
-    return (int)min((int64_t)tiles, (x - at) / ((int64_t)kKeyTile * a.group));
+    const int64_t read = x - at - (int64_t)kFixed * a.group;
+    return read <= 0 ? 0 : (int)min((int64_t)tiles, read / ((int64_t)kKeyTile * a.group));
   }
 
   __device__ __forceinline__ void advance() {

@@ -24,6 +24,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "runtime.h"
 
 namespace kvoff {
@@ -46,34 +48,75 @@ struct RotaryArgs {
   int32_t lanes, tokens_per_cta;
   float sign;       // of the sines: -1 for the transpose
   bool positions64, copy;  // copy: units that pass through are written too
+  bool wide_table;         // its rows' halves can be read 16 bytes at a time
 };
 
-template <typename T>
-__device__ __forceinline__ float to_f32(T x);
-template <>
-__device__ __forceinline__ float to_f32(float x) { return x; }
-template <>
-__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <>
-__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
-
-template <typename T>
-__device__ __forceinline__ T from_f32(float x);
-template <>
-__device__ __forceinline__ float from_f32(float x) { return x; }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32(float x) { return __float2bfloat16_rn(x); }
-template <>
-__device__ __forceinline__ __half from_f32(float x) { return __float2half_rn(x); }
-
+// V adjacent values of a row as they stand in memory, read and written as 32-bit
+// words where there is a whole one.
 template <typename T, int V>
-struct alignas(sizeof(T) * V) Vec {
-  T x[V];
+struct Vec {
+  static constexpr int kBytes = sizeof(T) * V;
+  uint32_t w[kBytes < 4 ? 1 : kBytes / 4];
+
+  __device__ __forceinline__ void load(const uint8_t* p) {
+    if constexpr (kBytes == 16) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p);
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else if constexpr (kBytes == 8) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      w[0] = v.x, w[1] = v.y;
+    } else if constexpr (kBytes == 4) {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else {
+      w[0] = *reinterpret_cast<const uint16_t*>(p);
+    }
+  }
+  __device__ __forceinline__ void store(uint8_t* p) const {
+    if constexpr (kBytes == 16)
+      *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    else if constexpr (kBytes == 8)
+      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else if constexpr (kBytes == 4)
+      *reinterpret_cast<uint32_t*>(p) = w[0];
+    else
+      *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[0];
+  }
+  __device__ __forceinline__ void unpack(float (&x)[V]) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[i] = __uint_as_float(w[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const uint32_t u = w[i / 2];
+        if constexpr (std::is_same<T, __half>::value)
+          x[i] = __half2float(__ushort_as_half((unsigned short)(i % 2 ? u >> 16 : u & 0xFFFFu)));
+        else
+          x[i] = __uint_as_float(i % 2 ? u & 0xFFFF0000u : u << 16);
+      }
+    }
+  }
+  __device__ __forceinline__ void pack(const float (&x)[V]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) w[i] = __float_as_uint(x[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; i += 2) {
+        const float low = x[i], high = V > 1 ? x[(i + 1) % V] : 0.0f;
+        if constexpr (std::is_same<T, __half>::value)
+          asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[i / 2]) : "f"(high), "f"(low));
+        else
+          asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i / 2]) : "f"(high), "f"(low));
+      }
+    }
+  }
 };
 
 // V values per vector; a unit is two vectors in the half layout, one else.
 template <typename T, int V, bool kInterleaved>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
+__global__ void __launch_bounds__(kThreads, 3)
+    rotary_kernel(const __grid_constant__ RotaryArgs a) {
   constexpr int kPairs = kInterleaved ? V / 2 : V;
   using Vector = Vec<T, V>;
   const int per_token = a.units * a.lanes;
@@ -81,61 +124,90 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
   const int rest = threadIdx.x % per_token;
   const int unit = rest % a.units, lane = rest / a.units;
   if (threadIdx.x >= a.tokens_per_cta * per_token || token >= a.num_tokens) return;
-  const int64_t position = a.positions64 ? static_cast<const int64_t*>(a.positions)[token]
-                                         : static_cast<const int32_t*>(a.positions)[token];
-  if (position < 0) return;
-  if (position >= a.table_rows) {
-    if (rest == 0 && a.bad_positions != nullptr) atomicAdd(a.bad_positions, 1);
-    return;
-  }
   const bool turns = unit < a.turning;
   if (!turns && !a.copy) return;
   const int half = a.rotary_dim / 2;
   // First value of the unit, and of its partner vector.
   const int at = turns ? unit * V : a.rotary_dim + (unit - a.turning) * V;
-  const int partner = (!kInterleaved && turns) ? at + half : at;
-  float c[kPairs], s[kPairs];
-  if (turns) {
-    const float* row = a.table + position * a.rotary_dim + unit * kPairs;
-#pragma unroll
-    for (int i = 0; i < kPairs; ++i) {
-      c[i] = __ldg(row + i);
-      s[i] = a.sign * __ldg(row + half + i);
-    }
-  }
+  const int partner = (!kInterleaved && turns) ? half : 0;
   const int heads = a.heads[0] + a.heads[1];
-  for (int first = lane; first < heads; first += kUnroll * a.lanes) {
-    Vector x[kUnroll], y[kUnroll];
+  const int row = a.dim * (int)sizeof(T);
+  const uint8_t* in_q = a.in[0] + token * a.in_stride[0] + at * sizeof(T);
+  const uint8_t* in_k = a.in[1] + token * a.in_stride[1] + at * sizeof(T) - a.heads[0] * row;
+  uint8_t* out_q = a.out[0] + token * a.out_stride[0] + at * sizeof(T);
+  uint8_t* out_k = a.out[1] + token * a.out_stride[1] + at * sizeof(T) - a.heads[0] * row;
+
+  const int64_t position = a.positions64 ? __ldg(static_cast<const long long*>(a.positions) + token)
+                                         : __ldg(static_cast<const int32_t*>(a.positions) + token);
+  // The first heads' values are on the way while the table row is looked up.
+  Vector x[kUnroll], y[kUnroll];
+  auto load = [&](int first) {
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) {
       const int h = first + i * a.lanes;
       if (h < heads) {
-        const bool is_k = h >= a.heads[0];
-        const uint8_t* p = (is_k ? a.in[1] + token * a.in_stride[1] : a.in[0] + token * a.in_stride[0]) +
-                           (int64_t)(is_k ? h - a.heads[0] : h) * a.dim * sizeof(T);
-        x[i] = *reinterpret_cast<const Vector*>(p + at * sizeof(T));
-        if (!kInterleaved) y[i] = *reinterpret_cast<const Vector*>(p + partner * sizeof(T));
+        const uint8_t* p = (h < a.heads[0] ? in_q : in_k) + h * row;
+        x[i].load(p);
+        if (!kInterleaved) y[i].load(p + partner * sizeof(T));
+      }
+    }
+  };
+  load(lane);
+  if (position < 0) return;
+  if (position >= a.table_rows) {
+    if (rest == 0 && a.bad_positions != nullptr) atomicAdd(a.bad_positions, 1);
+    return;
+  }
+  float c[kPairs], s[kPairs];
+  if (turns) {
+    const float* from = a.table + position * a.rotary_dim + unit * kPairs;
+    constexpr int kWide = kPairs % 4 == 0 ? 4 : 1;
+#pragma unroll
+    for (int i = 0; i < kPairs; i += kWide) {
+      if (kWide == 4 && a.wide_table) {
+        const float4 u = __ldg(reinterpret_cast<const float4*>(from + i));
+        const float4 v = __ldg(reinterpret_cast<const float4*>(from + half + i));
+        c[i] = u.x, c[i + kWide / 4] = u.y, c[i + kWide / 2] = u.z, c[i + kWide * 3 / 4] = u.w;
+        s[i] = v.x, s[i + kWide / 4] = v.y, s[i + kWide / 2] = v.z, s[i + kWide * 3 / 4] = v.w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < kWide; ++j) c[i + j] = __ldg(from + i + j), s[i + j] = __ldg(from + half + i + j);
       }
     }
 #pragma unroll
+    for (int i = 0; i < kPairs; ++i) s[i] *= a.sign;
+  }
+  for (int first = lane; first < heads; first += kUnroll * a.lanes) {
+    if (first != lane) load(first);
+#pragma unroll
     for (int i = 0; i < kUnroll; ++i) {
       const int h = first + i * a.lanes;
       if (h < heads) {
-        const bool is_k = h >= a.heads[0];
-        uint8_t* p = (is_k ? a.out[1] + token * a.out_stride[1] : a.out[0] + token * a.out_stride[0]) +
-                     (int64_t)(is_k ? h - a.heads[0] : h) * a.dim * sizeof(T);
+        uint8_t* p = (h < a.heads[0] ? out_q : out_k) + h * row;
         if (turns) {
+          float u[V], v[V];
+          x[i].unpack(u);
+          if (kInterleaved) {
 #pragma unroll
-          for (int j = 0; j < kPairs; ++j) {
-            T& first_of = kInterleaved ? x[i].x[2 * j] : x[i].x[j];
-            T& second_of = kInterleaved ? x[i].x[2 * j + 1] : y[i].x[j];
-            const float x1 = to_f32(first_of), x2 = to_f32(second_of);
-            first_of = from_f32<T>(x1 * c[j] - x2 * s[j]);
-            second_of = from_f32<T>(x2 * c[j] + x1 * s[j]);
+            for (int j = 0; j < kPairs; ++j) {
+              const float x1 = u[2 * j], x2 = u[2 * j + 1];
+              u[2 * j] = x1 * c[j] - x2 * s[j];
+              u[2 * j + 1] = x2 * c[j] + x1 * s[j];
+            }
+          } else {
+            y[i].unpack(v);
+#pragma unroll
+            for (int j = 0; j < kPairs; ++j) {
+              const float x1 = u[j], x2 = v[j];
+              u[j] = x1 * c[j] - x2 * s[j];
+              v[j] = x2 * c[j] + x1 * s[j];
+            }
+            y[i].pack(v);
+            y[i].store(p + partner * sizeof(T));
           }
-          if (!kInterleaved) *reinterpret_cast<Vector*>(p + partner * sizeof(T)) = y[i];
+          x[i].pack(u);
         }
-        *reinterpret_cast<Vector*>(p + at * sizeof(T)) = x[i];
+        x[i].store(p);
       }
     }
   }
@@ -245,6 +317,7 @@ extern "C" int kvoff_rotary(const void* q, int64_t q_stride_bytes, void* q_out,
   a.dim = (int32_t)head_dim;
   a.rotary_dim = (int32_t)rotary_dim;
   a.sign = (flags & KVOFF_ROTARY_INVERSE) != 0 ? -1.0f : 1.0f;
+  a.wide_table = rotary_dim % 8 == 0 && (reinterpret_cast<uintptr_t>(table) & 15u) == 0;
   a.copy = rotary_dim < head_dim &&
            ((q_heads > 0 && q != q_out) || (kv_heads > 0 && k != k_out));
   cudaStream_t s = static_cast<cudaStream_t>(stream);

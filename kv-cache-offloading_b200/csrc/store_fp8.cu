@@ -40,6 +40,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "codec.cuh"
 #include "runtime.h"
 
@@ -47,7 +49,9 @@ namespace kvoff {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kKept = 4;        // rows of a thread group held in registers between the passes
+constexpr int kKeptLarge = 8;   // rows of a thread group held in registers between the passes
+constexpr int kKeptSmall = 4;
+constexpr int kResident = 2;    // CTAs an SM: registers for the rows that are held
 constexpr int kWindow = 16;     // tokens a CTA looks at for the start of a run
 constexpr int64_t kSmallCall = 1024;  // up to here a CTA looks at one token
 constexpr int64_t kMostTokens = 65536;
@@ -62,67 +66,74 @@ struct StoreArgs {
   const int32_t* slots;
   int32_t* bad_slots;
   int64_t num_slots;
-  int32_t num_tokens, heads, dim, shift, pairs, window;
+  int32_t num_tokens, heads, dim, shift, pairs, pair_shift, window;
   bool wide_slots;  // slots can be read 16 bytes at a time
 };
 
+// Both rows' types order their magnitudes by their bits; from kInf on they are
+// infinities and NaN.
 template <typename T>
-__device__ __forceinline__ void unpack(const uint4& v, float (&x)[8]);
-template <>
-__device__ __forceinline__ void unpack<__nv_bfloat16>(const uint4& v, float (&x)[8]) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = __uint_as_float(w[i] << 16);
-    x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-  }
-}
-template <>
-__device__ __forceinline__ void unpack<__half>(const uint4& v, float (&x)[8]) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-    x[2 * i] = f.x;
-    x[2 * i + 1] = f.y;
-  }
+constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+
+template <typename T>
+__device__ __forceinline__ float2 unpack(uint32_t w) {
+  if constexpr (std::is_same<T, __half>::value)
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  else
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
 }
 
-// Bits of the largest finite magnitude among the values, and `most`.
-__device__ __forceinline__ uint32_t finite_amax(const float (&x)[8], uint32_t most) {
-#pragma unroll
+// Magnitude bits (16) of the largest of the eight values.
+__device__ __forceinline__ uint32_t largest(const uint4& v) {
+  constexpr uint32_t m = 0x7FFF7FFFu;
+  const uint32_t x = __vmaxu2(__vmaxu2(v.x & m, v.y & m), __vmaxu2(v.z & m, v.w & m));
+  return max(x & 0xFFFFu, x >> 16);
+}
+
+// The same among the finite values.
+template <typename T>
+__device__ __noinline__ uint32_t largest_finite(uint4 v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t most = 0;
   for (int i = 0; i < 8; ++i) {
-    const uint32_t m = __float_as_uint(x[i]) & 0x7FFFFFFFu;
-    if (m < 0x7F800000u) most = max(most, m);
+    const uint32_t m = w[i / 2] >> i % 2 * 16 & 0x7FFFu;
+    if (m < kInf<T>) most = max(most, m);
   }
   return most;
 }
 
 // The smallest power of two s with amax <= 448 s = 1.75 * 2^8 s, at least 2^kMinExponent.
-__device__ __forceinline__ float scale_for(uint32_t amax_bits) {
-  int e = (int)(amax_bits >> 23) - 127 - 8 + ((amax_bits & 0x7FFFFFu) > 0x600000u);
+template <typename T>
+__device__ __forceinline__ float scale_for(uint32_t amax16) {
+  const uint32_t bits = __float_as_uint(unpack<T>(amax16).x);
+  int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7FFFFFu) > 0x600000u);
   e = max(e, kMinExponent);
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
-// x / scale as e4m3 bytes. The reciprocal of a power of two is exact; another
-// scale (one that the caller put there) is divided by.
-__device__ __forceinline__ uint2 encode(const float (&x)[8], float scale) {
-  float y[8];
-  if ((__float_as_uint(scale) & 0x7FFFFFu) == 0) {
-    const float r = __fdiv_rn(1.0f, scale);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = x[i] * r;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = __fdiv_rn(x[i], scale);
+// x / scale as e4m3 bytes, NaN where x is not finite. The reciprocal of a power
+// of two is exact; another scale (one that the caller put there) is divided by.
+template <typename T>
+__device__ __noinline__ uint2 encode_any(uint4 v, float scale) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t out[4];
+  for (int i = 0; i < 4; ++i) {
+    const float2 x = unpack<T>(w[i]);
+    const float nan = __uint_as_float(0x7FC00000u);
+    const float lo = (w[i] & 0x7FFFu) < kInf<T> ? __fdiv_rn(x.x, scale) : nan;
+    const float hi = (w[i] >> 16 & 0x7FFFu) < kInf<T> ? __fdiv_rn(x.y, scale) : nan;
+    out[i] = f32x2_to_e4m3x2(lo, hi);
   }
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if ((__float_as_uint(x[i]) & 0x7FFFFFFFu) >= 0x7F800000u) y[i] = __uint_as_float(0x7FC00000u);
+  return make_uint2(out[0] | out[1] << 16, out[2] | out[3] << 16);
+}
+
+template <typename T>
+__device__ __forceinline__ uint2 encode_finite(const uint4& v, float reciprocal) {
+  const float2 a = unpack<T>(v.x), b = unpack<T>(v.y), c = unpack<T>(v.z), d = unpack<T>(v.w);
+  const float r = reciprocal;
   uint2 out;
-  out.x = f32x2_to_e4m3x2(y[0], y[1]) | f32x2_to_e4m3x2(y[2], y[3]) << 16;
-  out.y = f32x2_to_e4m3x2(y[4], y[5]) | f32x2_to_e4m3x2(y[6], y[7]) << 16;
+  out.x = f32x2_to_e4m3x2(a.x * r, a.y * r) | f32x2_to_e4m3x2(b.x * r, b.y * r) << 16;
+  out.y = f32x2_to_e4m3x2(c.x * r, c.y * r) | f32x2_to_e4m3x2(d.x * r, d.y * r) << 16;
   return out;
 }
 
@@ -137,136 +148,192 @@ __device__ __forceinline__ uint2 rescale(const uint2& payload, float factor) {
   return out;
 }
 
-template <typename T, int LANES>
-__global__ void __launch_bounds__(kThreads) store_kvcache_fp8_kernel(const StoreArgs a) {
+template <typename T>
+__device__ __forceinline__ uint4 load_row(const uint8_t* p) {
+  uint4 v;  // read once: kept out of L1, which holds the slots
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+template <typename T, int LANES, int kKept>
+__global__ void __launch_bounds__(kThreads, kResident)
+    store_kvcache_fp8_kernel(const __grid_constant__ StoreArgs a) {
   constexpr int kGroups = kThreads / LANES;
-  extern __shared__ int32_t shared[];
-  __shared__ int32_t window[kWindow + 1];
+  extern __shared__ int32_t winner[];  // last token that writes each row of the block, or -1
+  __shared__ int32_t window[kWindow];
+  __shared__ uint32_t starts;
   __shared__ uint32_t amax[kGroups];
-  __shared__ int32_t count, earlier;
-  const int block = 1 << a.shift;
-  int32_t* winner = shared;          // last token that writes each row of the block, or -1
-  int32_t* written = shared + block;  // the rows that have one
-  const int tid = threadIdx.x, lane = tid % LANES;
-  const int mine = (tid / LANES) % a.pairs;  // this thread's pair among the CTA's
-  const int sub = (tid / LANES) / a.pairs, subs = kGroups / a.pairs;
-  const int pair = blockIdx.y * a.pairs + mine;
-  const bool active = pair < 2 * a.heads && lane * 8 < a.dim;
-  const int kv = pair >= a.heads ? 1 : 0, head = pair - kv * a.heads;
-  const int64_t row_bytes = (int64_t)a.heads * a.dim;
+  __shared__ int32_t earlier, far;
+  const int tid = threadIdx.x;
   const int first = blockIdx.x * a.window;
 
-  // slot_mapping[first - 1 .. first + window): is a token the start of a run?
-  if (tid <= a.window) {
-    const int i = first - 1 + tid;
+  // Which of the CTA's tokens begin a run: those whose nearest token before
+  // them, skipped ones left out, is in another block (or is not looked at).
+  if (tid < 32) {
+    const int i = first - (32 - kWindow) + tid;  // lanes 16 .. 16 + window: the CTA's tokens
+    const bool own = tid >= 32 - kWindow && tid < 32 - kWindow + a.window;
     int32_t slot = -1;
-    if (i >= 0 && i < a.num_tokens) slot = a.slots[i];
+    if (i >= 0 && i < a.num_tokens) slot = __ldg(a.slots + i);
     if (slot >= a.num_slots) {
-      if (tid > 0 && blockIdx.y == 0 && a.bad_slots != nullptr) atomicAdd(a.bad_slots, 1);
+      if (own && blockIdx.y == 0 && a.bad_slots != nullptr) atomicAdd(a.bad_slots, 1);
       slot = -1;
     }
-    window[tid] = slot < 0 ? -1 : slot >> a.shift;
+    const int32_t id = slot < 0 ? -1 : slot >> a.shift;
+    const uint32_t before = __ballot_sync(0xFFFFFFFFu, id >= 0) & ((1u << tid) - 1);
+    const int32_t previous = __shfl_sync(0xFFFFFFFFu, id, before == 0 ? 0 : 31 - __clz(before));
+    const bool start = own && id >= 0 && (before == 0 || previous != id);
+    const uint32_t mask = __ballot_sync(0xFFFFFFFFu, start) >> (32 - kWindow);
+    if (own) window[tid - (32 - kWindow)] = id;
+    if (tid == 0) starts = mask;
   }
   __syncthreads();
+  uint32_t todo = starts;
+  if (todo == 0) return;
 
-  for (int w = 1; w <= a.window; ++w) {
+  const uint32_t block = 1u << a.shift;
+  const int lane = tid % LANES;
+  const int mine = (tid / LANES) & (a.pairs - 1);  // this thread's pair among the CTA's
+  const int subs = kGroups >> a.pair_shift, sub = (tid / LANES) >> a.pair_shift;
+  const int pair = blockIdx.y * a.pairs + mine;
+  const bool active = pair < 2 * a.heads && lane * 8 < a.dim;
+  const bool is_v = pair >= a.heads;
+  const int head = is_v ? pair - a.heads : pair;
+  const int64_t row_bytes = (int64_t)a.heads * a.dim;
+  const int64_t stride = is_v ? a.stride[1] : a.stride[0];
+  const uint8_t* source =
+      (is_v ? a.rows[1] : a.rows[0]) + ((int64_t)head * a.dim + lane * 8) * sizeof(T);
+  for (; todo != 0; todo &= todo - 1) {
+    const int w = __ffs(todo) - 1, leader = first + w;
     const int32_t id = window[w];
-    if (id < 0 || id == window[w - 1]) continue;  // the same decision in all threads
-    const int leader = first + w - 1;
-    for (int i = tid; i < block; i += kThreads) winner[i] = -1;
+    for (int i = tid; i < (int)block; i += kThreads) winner[i] = -1;
     if (tid < a.pairs) amax[tid] = 0;
-    if (tid == 0) count = earlier = 0;
+    if (tid == 0) earlier = far = 0;
     __syncthreads();
-    const int64_t base = (int64_t)id << a.shift;
+    const int32_t base = id << a.shift;
+    // A slot's row in the block, or a number not below `block`.
+    auto row_of = [&](int32_t slot) { return (uint32_t)slot - (uint32_t)base; };
+    // The rows of the run, which are nearly always all of the block's: this
+    // thread's are on the way while the other slots are looked at.
+    uint4 kept[kKept];
+    int32_t offset[kKept];
+#pragma unroll
+    for (int i = 0; i < kKept; ++i) {
+      const int r = sub + i * subs, token = leader + r;
+      offset[i] = -1;
+      if (r < (int)block && token < a.num_tokens) {
+        const uint32_t row = row_of(__ldg(a.slots + token));
+        if (row < block) {
+          offset[i] = (int32_t)row;
+          if (active) kept[i] = load_row<T>(source + token * stride);
+        }
+      }
+    }
     auto look = [&](int i, int32_t slot) {
-      if (slot >= 0 && slot >> a.shift == id) {
-        if (i < leader)
+      if (row_of(slot) < block) {
+        if (i < leader) {
           earlier = 1;
-        else
-          atomicMax(&winner[slot - (int32_t)base], i);
+        } else {
+          atomicMax(&winner[row_of(slot)], i);
+          if (i >= leader + (int)block) far = 1;
+        }
       }
     };
     if (a.wide_slots) {
       const int quads = a.num_tokens / 4;
+#pragma unroll 4
       for (int i = tid; i < quads; i += kThreads) {
         const int4 s = __ldg(reinterpret_cast<const int4*>(a.slots) + i);
-        look(4 * i, s.x);
-        look(4 * i + 1, s.y);
-        look(4 * i + 2, s.z);
-        look(4 * i + 3, s.w);
+        if (min(min(row_of(s.x), row_of(s.y)), min(row_of(s.z), row_of(s.w))) < block) {
+          look(4 * i, s.x);
+          look(4 * i + 1, s.y);
+          look(4 * i + 2, s.z);
+          look(4 * i + 3, s.w);
+        }
       }
       for (int i = 4 * quads + tid; i < a.num_tokens; i += kThreads) look(i, __ldg(a.slots + i));
     } else {
       for (int i = tid; i < a.num_tokens; i += kThreads) look(i, __ldg(a.slots + i));
     }
+    float* scale = (is_v ? a.scale[1] : a.scale[0]) + (int64_t)id * a.heads + head;
+    float before = 0.0f;
+    if (active) before = *scale;
     __syncthreads();
     if (earlier != 0) {  // another CTA owns the block
       __syncthreads();
       continue;
     }
-    for (int i = tid; i < block; i += kThreads)
-      if (winner[i] >= 0) written[atomicAdd(&count, 1)] = i;
     const bool opened = winner[0] >= 0;
-    float* scale = (kv != 0 ? a.scale[1] : a.scale[0]) + (int64_t)id * a.heads + head;
-    float old = 0.0f;
-    if (active && !opened) {
-      old = *scale;
-      if (!(old > 0.0f && __float_as_uint(old) < 0x7F800000u)) old = 0.0f;
-    }
-    __syncthreads();
+    const float old =
+        !opened && before > 0.0f && __float_as_uint(before) < 0x7F800000u ? before : 0.0f;
 
-    const int rows = count;
-    const int64_t stride = kv != 0 ? a.stride[1] : a.stride[0];
-    const uint8_t* source =
-        (kv != 0 ? a.rows[1] : a.rows[0]) + ((int64_t)head * a.dim + lane * 8) * sizeof(T);
-    uint8_t* target = (kv != 0 ? a.cache[1] : a.cache[0]) + base * row_bytes + (int64_t)head * a.dim + lane * 8;
+    uint8_t* target = (is_v ? a.cache[1] : a.cache[0]) + base * row_bytes +
+                      (int64_t)head * a.dim + lane * 8;
+    // Calls f(row, offset) for this thread's rows that are not in `kept`: the
+    // rest of the run, and rows of the block from further on in the call.
+    auto others = [&](auto f) {
+      constexpr int kBatch = 4;  // loads in flight
+      for (int r = sub + kKept * subs; r < (int)block; r += kBatch * subs) {
+        uint4 row[kBatch];
+        int at[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int token = leader + r + i * subs;
+          at[i] = -1;
+          if (r + i * subs < (int)block && token < a.num_tokens) {
+            const uint32_t to = row_of(__ldg(a.slots + token));
+            if (to < block && winner[to] == token) {
+              at[i] = (int)to;
+              row[i] = load_row<T>(source + token * stride);
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+          if (at[i] >= 0) f(row[i], at[i]);
+      }
+      if (far != 0)
+        for (int r = sub; r < (int)block; r += subs)
+          if (winner[r] >= leader + (int)block) f(load_row<T>(source + winner[r] * stride), r);
+    };
     uint32_t most = 0;
-    uint4 kept[kKept];
+    bool finite = true;
+    auto size_of = [&](const uint4& row) {
+      const uint32_t size = largest(row);
+      if (size < kInf<T>) return size;
+      finite = false;
+      return largest_finite<T>(row);
+    };
     if (active) {
 #pragma unroll
       for (int i = 0; i < kKept; ++i) {
-        const int r = sub + i * subs;
-        if (r < rows)
-          kept[i] = *reinterpret_cast<const uint4*>(source + winner[written[r]] * stride);
-      }
-#pragma unroll
-      for (int i = 0; i < kKept; ++i)
-        if (sub + i * subs < rows) {
-          float x[8];
-          unpack<T>(kept[i], x);
-          most = finite_amax(x, most);
+        if (offset[i] >= 0 && winner[offset[i]] != leader + sub + i * subs) offset[i] = -1;
+        if (offset[i] >= 0) {
+          most = max(most, size_of(kept[i]));
         }
-#pragma unroll 4
-      for (int r = sub + kKept * subs; r < rows; r += subs) {
-        float x[8];
-        unpack<T>(*reinterpret_cast<const uint4*>(source + winner[written[r]] * stride), x);
-        most = finite_amax(x, most);
       }
+      others([&](const uint4& row, int) { most = max(most, size_of(row)); });
     }
 #pragma unroll
     for (int d = LANES / 2; d > 0; d /= 2) most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
     if (lane == 0 && most != 0) atomicMax(&amax[mine], most);
     __syncthreads();
     if (active) {
-      const float now = fmaxf(scale_for(amax[mine]), old);
+      const float now = fmaxf(scale_for<T>(amax[mine]), old);
+      const float reciprocal = __fdiv_rn(1.0f, now);
+      const bool plain = finite && (__float_as_uint(now) & 0x7FFFFFu) == 0;
+      auto put = [&](const uint4& row, int at) {
+        *reinterpret_cast<uint2*>(target + at * row_bytes) =
+            plain ? encode_finite<T>(row, reciprocal) : encode_any<T>(row, now);
+      };
 #pragma unroll
-      for (int i = 0; i < kKept; ++i) {
-        const int r = sub + i * subs;
-        if (r < rows) {
-          float x[8];
-          unpack<T>(kept[i], x);
-          *reinterpret_cast<uint2*>(target + written[r] * row_bytes) = encode(x, now);
-        }
-      }
-#pragma unroll 4
-      for (int r = sub + kKept * subs; r < rows; r += subs) {
-        float x[8];
-        unpack<T>(*reinterpret_cast<const uint4*>(source + winner[written[r]] * stride), x);
-        *reinterpret_cast<uint2*>(target + written[r] * row_bytes) = encode(x, now);
-      }
+      for (int i = 0; i < kKept; ++i)
+        if (offset[i] >= 0) put(kept[i], offset[i]);
+      others(put);
       if (!opened && now != old) {
         const float factor = __fdiv_rn(old, now);
-        for (int r = sub; r < block; r += subs)
+        for (int r = sub; r < (int)block; r += subs)
           if (winner[r] < 0) {
             uint2* p = reinterpret_cast<uint2*>(target + r * row_bytes);
             *p = rescale(*p, factor);
@@ -278,7 +345,7 @@ __global__ void __launch_bounds__(kThreads) store_kvcache_fp8_kernel(const Store
   }
 }
 
-template <typename T, int LANES>
+template <typename T, int LANES, int kKept>
 int launch(StoreArgs a, cudaStream_t stream) {
   constexpr int kGroups = kThreads / LANES;
   const int block = 1 << a.shift;
@@ -290,21 +357,28 @@ int launch(StoreArgs a, cudaStream_t stream) {
                              : (a.num_tokens + block - 1) / block;
   int pairs = 1;
   while (pairs < kGroups && pairs < 2 * a.heads) pairs *= 2;
-  while (pairs > 1 && blocks * ((2 * a.heads + pairs - 1) / pairs) < 4 * sm_count()) pairs /= 2;
+  while (pairs > 1 && blocks * ((2 * a.heads + pairs - 1) / pairs) < 2 * sm_count()) pairs /= 2;
+  while (pairs > 1 && kGroups / pairs * kKept < block) pairs /= 2;
   a.pairs = pairs;
+  while ((1 << a.pair_shift) < pairs) ++a.pair_shift;
   const dim3 grid((a.num_tokens + a.window - 1) / a.window, (2 * a.heads + pairs - 1) / pairs);
-  store_kvcache_fp8_kernel<T, LANES>
-      <<<grid, kThreads, 2 * block * sizeof(int32_t), stream>>>(a);
+  store_kvcache_fp8_kernel<T, LANES, kKept>
+      <<<grid, kThreads, block * sizeof(int32_t), stream>>>(a);
   return cuda_status(cudaGetLastError(), "store_kvcache_fp8 launch");
+}
+
+template <typename T, int LANES>
+int launch_kept(const StoreArgs& a, cudaStream_t stream) {
+  return a.num_tokens <= kSmallCall ? launch<T, LANES, kKeptSmall>(a, stream) : launch<T, LANES, kKeptLarge>(a, stream);
 }
 
 template <typename T>
 int launch_lanes(const StoreArgs& a, cudaStream_t stream) {
   const int vectors = a.dim / 8;
-  if (vectors <= 4) return launch<T, 4>(a, stream);
-  if (vectors <= 8) return launch<T, 8>(a, stream);
-  if (vectors <= 16) return launch<T, 16>(a, stream);
-  return launch<T, 32>(a, stream);
+  if (vectors <= 4) return launch_kept<T, 4>(a, stream);
+  if (vectors <= 8) return launch_kept<T, 8>(a, stream);
+  if (vectors <= 16) return launch_kept<T, 16>(a, stream);
+  return launch_kept<T, 32>(a, stream);
 }
 
 }  // namespace
