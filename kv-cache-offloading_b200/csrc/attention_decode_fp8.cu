@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_decode_fp8_kernel(const
 
   Walk<kThreads> walk(a, &walk_shared);
   Segment seg;
-  while (walk.next(&seg)) {
+  while (walk.next(a, &seg)) {
     const Sequence& seq = walk.seq;
     Rows<D, NT> r;
     load_rows<D, NT>(a, seq, seg, g, t, r);
@@ -546,9 +546,9 @@ __global__ void __launch_bounds__(kThreads, 2) attention_decode_fp8_kernel(const
       }
     }
     __syncthreads();  // the sums are read before the next segment fills the rings
-    walk.advance();
+    walk.advance(a);
   }
-  walk.finish();
+  if (threadIdx.x == 0) walk.finish(a);
 }
 
 template <int D, int NT>
@@ -566,10 +566,6 @@ int launch(const Args& a, int grid, cudaStream_t stream) {
 }
 
 }  // namespace
-
-int decode_grid() { return 2 * sm_count(); }
-
-int decode_rows(int64_t rows) { return rows <= 8 ? 8 : kDecodeRows; }
 
 int launch_decode(const Args& a, int dim, int grid, cudaStream_t stream) {
   if (dim == 128) return a.rows == 8 ? launch<128, 1>(a, grid, stream) : launch<128, 2>(a, grid, stream);

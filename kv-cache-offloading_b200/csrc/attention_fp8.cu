@@ -84,17 +84,18 @@ struct Shape {
 struct Choice {
   int rows, grid;
   int64_t max_tiles;
-  bool direct;
+  bool direct, extend;
 };
 
 Choice choose(const Shape& s) {
   Choice c{};
   const int64_t rows = s.max_q * (s.q_heads / s.kv_heads);
-  c.rows = decode_rows(rows);
+  c.extend = rows > kDecodeRows;
+  c.rows = c.extend ? kExtendRows : rows <= 8 ? 8 : kDecodeRows;
   c.max_tiles = (rows + c.rows - 1) / c.rows;
   const int64_t ctas = s.seqs * s.kv_heads * c.max_tiles;
   c.direct = s.keys <= kDirectKeys && ctas <= 0x7FFFFFFFll;
-  c.grid = c.direct ? (int)ctas : decode_grid();
+  c.grid = c.direct ? (int)ctas : c.extend ? sm_count() : 2 * sm_count();
   return c;
 }
 
@@ -164,6 +165,8 @@ extern "C" int kvoff_attention_fp8(
     return fail(KVOFF_EINVAL, "kvoff_attention_fp8: without cu_seqlens_q each sequence has one token");
   if (num_tokens > 0x7FFFFFFFll / q_heads)
     return fail(KVOFF_EINVAL, "kvoff_attention_fp8: sizes exceed 32 bits");
+  if (!(softmax_scale > 0.0f && softmax_scale < 3.4e38f))
+    return fail(KVOFF_EINVAL, "kvoff_attention_fp8: softmax_scale must be positive and finite");
   if (num_seqs == 0 || num_tokens == 0 || max_seqlen_q == 0) return ok();
   if (q == nullptr || out == nullptr || context_lens == nullptr ||
       (s.keys > 0 && (k_cache == nullptr || v_cache == nullptr || k_scale == nullptr ||
@@ -206,14 +209,17 @@ extern "C" int kvoff_attention_fp8(
   a.kv_heads = (int32_t)kv_heads;
   a.group = (int32_t)(q_heads / kv_heads);
   a.rows = c.rows;
+  a.fixed = c.extend ? attention::kExtendFixed : attention::kDecodeFixed;
   a.max_tiles = (int32_t)c.max_tiles;
   a.direct = c.direct;
   a.bf16 = dtype == KVOFF_BF16;
+  a.wide_out = (pairs & 15u) == 0;
   a.records = static_cast<attention::Record*>(workspace);
   a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
                                        c.grid * (int64_t)sizeof(attention::Record));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  KVOFF_TRY(attention::launch_decode(a, (int)head_dim, c.grid, st));
+  KVOFF_TRY(c.extend ? attention::launch_extend(a, (int)head_dim, c.grid, st)
+                     : attention::launch_decode(a, (int)head_dim, c.grid, st));
   if (!c.direct) KVOFF_TRY(attention::launch_join(a, (int)head_dim, c.grid, st));
   return ok();
 }

@@ -14,10 +14,6 @@ namespace attention {
 
 // Keys of one step of the partition.
 constexpr int kKeyTile = 128;
-// What beginning and ending a row tile costs, as keys read: 4.3 us, against
-// 0.5 us a tile of 128 keys. Without it a CTA that gets a hundred short
-// sequences ends last (64 sequences of 0 to 8192 keys: 243 us against 49).
-constexpr int kFixed = 768;
 
 struct Args {
   const uint8_t* q;
@@ -34,9 +30,11 @@ struct Args {
   int32_t table_width, num_pages, page, block_tiles;  // scale block in 16-key units
   int32_t seqs, num_tokens, q_heads, kv_heads, group;
   int32_t rows;      // packed rows of a row tile
+  int32_t fixed;     // what beginning and ending a row tile costs, as keys read
   int32_t max_tiles; // row tiles of the longest sequence (direct form)
   bool direct;       // one CTA per (sequence, head, row tile), nothing is split
   bool bf16;
+  bool wide_out;     // rows of out can be written 16 bytes at a time
   float* partial;            // 2 slots per CTA
   struct Record* records;    // one per CTA
 };
@@ -70,7 +68,7 @@ struct Sequence {
     context = (int32_t)min((int64_t)max(a.contexts[s], 0), room);
     const int64_t rows = (int64_t)q_len * a.group;
     tiles = (int32_t)((rows + a.rows - 1) / a.rows);
-    base = (int64_t)(max(context - q_len, 0) + kFixed) * a.group;
+    base = (int64_t)(max(context - q_len, 0) + a.fixed) * a.group;
   }
   __device__ __forceinline__ int64_t cost(const Args& a, int r) const {
     return base + min((int64_t)(r + 1) * a.rows, (int64_t)q_len * a.group);
@@ -103,10 +101,9 @@ struct Segment {
 // long sequence, keeps all SMs busy to the end, from lengths that only the
 // device knows. A triple that is cut is joined by join_kernel.
 //
-//   Walk walk(args); if walk.next(segment) ... until false; walk.finish().
+//   Walk walk(args); while (walk.next(segment)) { ...; walk.advance(); } walk.finish() once a CTA.
 template <int kThreads>
 struct Walk {
-  const Args& a;
   Sequence seq;
   int s, head, tile, cta;
   int64_t at, from, to, share;  // axis position of the triple; the CTA's stretch
@@ -119,7 +116,8 @@ struct Walk {
     int32_t seq;
   };
 
-  __device__ __forceinline__ Walk(const Args& args, Shared* sh) : a(args) {
+  Walk() = default;
+  __device__ __forceinline__ Walk(const Args& a, Shared* sh) {
     cta = blockIdx.x;
     record.further = -1;
     record.valid[0] = record.valid[1] = 0;
@@ -154,7 +152,7 @@ struct Walk {
       total += sh->warp_sum[i];
     }
     // A stretch of less than two key tiles costs more to join than to read.
-    const int64_t least = (int64_t)(2 * kKeyTile + kFixed) * a.group;
+    const int64_t least = (int64_t)(2 * kKeyTile + a.fixed) * a.group;
     share = max((total + gridDim.x - 1) / gridDim.x, least);
     from = cta * share;
     to = min(from + share, total);
@@ -193,13 +191,13 @@ struct Walk {
   }
 
   // The key tile at which the axis position x cuts the current triple.
-  __device__ __forceinline__ int cut(int64_t x, int64_t cost, int tiles) const {
+  __device__ __forceinline__ int cut(const Args& a, int64_t x, int64_t cost, int tiles) const {
     if (x >= at + cost) return tiles;
-    const int64_t read = x - at - (int64_t)kFixed * a.group;
+    const int64_t read = x - at - (int64_t)a.fixed * a.group;
     return read <= 0 ? 0 : (int)min((int64_t)tiles, read / ((int64_t)kKeyTile * a.group));
   }
 
-  __device__ __forceinline__ void advance() {
+  __device__ __forceinline__ void advance(const Args& a) {
     if (a.direct) {  // more row tiles than announced: the same CTAs take them
       tile += a.max_tiles;
       more = tile < seq.tiles;
@@ -215,7 +213,7 @@ struct Walk {
     while (seq.tiles == 0);
   }
 
-  __device__ __forceinline__ bool next(Segment* out) {
+  __device__ __forceinline__ bool next(const Args& a, Segment* out) {
     while (more) {
       out->seq = s;
       out->head = head;
@@ -227,8 +225,8 @@ struct Walk {
       out->slot = 0;
       if (!a.direct) {
         const int64_t cost = seq.cost(a, tile);
-        out->begin = cut(from, cost, out->tiles);
-        out->end = cut(to, cost, out->tiles);
+        out->begin = cut(a, from, cost, out->tiles);
+        out->end = cut(a, to, cost, out->tiles);
         out->slot = at >= from ? 1 : 0;
         out->whole = out->begin == 0 && out->end == out->tiles;
         const bool part = !out->whole && out->begin < out->end;
@@ -244,13 +242,13 @@ struct Walk {
         out->whole = true;
       }
       if (out->begin < out->end) return true;
-      advance();
+      advance(a);
     }
     return false;
   }
 
-  __device__ __forceinline__ void finish() {
-    if (!a.direct && threadIdx.x == 0) a.records[cta] = record;
+  __device__ __forceinline__ void finish(const Args& a) const {
+    if (!a.direct) a.records[cta] = record;
   }
 };
 
@@ -287,10 +285,20 @@ __device__ __forceinline__ void write_lse(const Args& a, int token, int q_head, 
 int launch_join(const Args& a, int dim, int grid, cudaStream_t stream);
 
 // The kernels. `dim` is 64 or 128; a is filled but for rows and partial.
-constexpr int kDecodeRows = 16;
-int decode_grid();
-int decode_rows(int64_t rows);  // rows of a row tile for `rows` packed rows a head
+// Rows are packed rows of a KV head: query tokens times `group`.
+constexpr int kDecodeRows = 16;   // the most of one row tile
+constexpr int kExtendRows = 256;
+// Beginning and ending a row tile of a decode step takes 4.3 us, against 0.5
+// us a tile of 128 keys. Without it in the partition a CTA that gets a hundred
+// short sequences ends last (64 sequences of 0 to 8192 keys: 243 us against 49).
+constexpr int kDecodeFixed = 768;
+constexpr int kExtendFixed = 512;
 int launch_decode(const Args& a, int dim, int grid, cudaStream_t stream);
+int launch_extend(const Args& a, int dim, int grid, cudaStream_t stream);
+
+// Error flags of extend's bounded waits on the current device.
+int extend_device_error(int32_t* flags, bool clear);
+constexpr int kErrExtendWaitTimeout = 2;
 
 }  // namespace attention
 }  // namespace kvoff

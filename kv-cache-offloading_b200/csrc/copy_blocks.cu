@@ -18,6 +18,7 @@
 
 #include <mutex>
 
+#include "attention_fp8.h"
 #include "runtime.h"
 
 namespace kvoff {
@@ -525,6 +526,7 @@ int kvoff_device_error(int32_t device, int32_t* flags, int32_t clear) {
     rc = cuda_status(cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int)),
                      "cudaMemcpyToSymbol (error flags)");
   }
+  if (rc == KVOFF_OK) rc = attention::extend_device_error(&value, clear != 0);
   cudaSetDevice(prev);
   if (rc != KVOFF_OK) return rc;
   *flags = value;
