@@ -12,6 +12,7 @@
 //   warps 0-3, 4-7  softmax of row tile 0 and 1, one row a thread
 //   warps 8-11      cache -> registers -> f16 operands in shared memory
 //   warp 12         one thread issues all matrix products
+//   warp 13         one thread walks the CTA's part of the work
 //
 // K, V and Q are f16 operands: e4m3 is a subset of f16, and q is scaled by a
 // power of two to an amax of 2^14..2^15, where every bf16 value down to 2^-31
@@ -44,11 +45,12 @@ constexpr int kThreads = 512;
 constexpr int kGroupRows = 128;    // rows of a tensor tile
 constexpr int kStages = 2;         // of K and of V
 constexpr int kScaleRing = 4;      // scales live longer than K's stage
+constexpr int kWorkRing = 2;       // segments handed out ahead
 constexpr float kRaise = 6.0f;     // log2 of how far P may pass 1
 constexpr float kWeightLog2 = 8.0f;
 constexpr float kLeastLog2 = -42.0f;  // of a V scale against the largest: P rounds to 0 in f16
 constexpr uint32_t kNegInf = 0xFF800000u;
-constexpr uint64_t kWaitLimitNs = 1000000000ull;
+constexpr uint32_t kWaitNs = 1000, kMostWaits = 1u << 20;  // a second in all
 constexpr uint32_t kTmemColumns = 512;
 constexpr uint32_t kScoresAt = 0, kOutputsAt = 256, kGroupColumns = 128;
 
@@ -63,10 +65,34 @@ struct Layout {
   static constexpr int kBytes = kNan + kStages * kNanBytes + 1024;  // 1024: alignment
 };
 
+// Of a tile's 16-key groups. The scale of V is a fraction of the largest one
+// that the segment has met, times 2^8: it is added to the exponent of P, and
+// its inverse takes it out of the sum of p again.
 struct Scales {
-  float k[8];       // of the tile's 16-key groups
-  float v_log2[8];
-  uint32_t absent;  // bit g: group g has no page
+  float k[8];
+  float shift[8];    // log2
+  float inverse[8];
+  float largest;     // log2 of the largest scale of V so far
+  uint32_t absent;   // bit g: group g has no page
+};
+
+// One segment, as the roles need it.
+struct Work {
+  int32_t begin, end;  // key tiles; end < 0: no more work
+  int32_t seq, head;
+  int32_t slot;        // of the partial result, -1 when the segment is whole
+  int32_t start;       // of the sequence's tokens
+  int32_t offset;      // context - q_len: token t sees offset + t + 1 keys
+  int32_t first_row, rows;
+  int32_t keys;        // that the last row sees: nothing is read behind them
+  int32_t fewest;      // that the first row sees
+  int32_t pad;
+
+  __device__ __forceinline__ int groups() const { return rows > 128 ? 2 : 1; }
+  // Whether rows see key tile `tile` to different lengths.
+  __device__ __forceinline__ bool mixed(int tile) const {
+    return (tile + 1) * kKeyTile > fewest && fewest < keys;
+  }
 };
 
 struct Shared {
@@ -78,13 +104,9 @@ struct Shared {
   uint32_t nan[kStages];  // n + 1: V of tile n, in this stage, holds NaN that some row must not meet
   uint32_t tmem;
   int32_t abort;
+  uint64_t work_full[kWorkRing], work_empty[kWorkRing];
+  Work work[kWorkRing];
   Walk<kThreads>::Shared walk;
-  // Each warp's place in the CTA's work, here rather than in registers: one
-  // lane moves it, once a segment.
-  struct Place {
-    Walk<kThreads> walk;
-    Segment segment;
-  } place[kThreads / 32];
 };
 
 __device__ __forceinline__ uint32_t smem_of(const void* p) {
@@ -101,32 +123,26 @@ __device__ __forceinline__ bool bar_try(uint64_t* bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(done)
-      : "r"(smem_of(bar)), "r"(parity)
+      : "r"(smem_of(bar)), "r"(parity), "r"(kWaitNs)
       : "memory");
   return done != 0;
 }
 
-// Waits for the phase of `parity`, at most kWaitLimitNs and not once another
-// role has given up. False: leave.
-__device__ __noinline__ bool bar_wait_slow(uint64_t* bar, uint32_t parity, int32_t* abort) {
-  uint64_t begin, now;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(begin));
-  for (uint32_t spins = 0; spins < 1u << 26; ++spins) {
-    if (bar_try(bar, parity)) return true;
-    if (*reinterpret_cast<volatile int32_t*>(abort) != 0) return false;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
-    if (now - begin > kWaitLimitNs) break;
-  }
-  *reinterpret_cast<volatile int32_t*>(abort) = 1;
-  atomicOr(&g_extend_error, kErrExtendWaitTimeout);
-  return false;
-}
+// Waits for the phase of `parity`, at most kMostWaits times kWaitNs and not
+// once another role has given up. False: leave.
 __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, int32_t* abort) {
-  if (bar_try(bar, parity)) return true;
-  return bar_wait_slow(bar, parity, abort);
+  for (uint32_t i = 0; !bar_try(bar, parity); ++i) {
+    if (*reinterpret_cast<volatile int32_t*>(abort) != 0) return false;
+    if (i >= kMostWaits) {
+      *reinterpret_cast<volatile int32_t*>(abort) = 1;
+      atomicOr(&g_extend_error, kErrExtendWaitTimeout);
+      return false;
+    }
+  }
+  return true;
 }
 // The same for a whole warp, whose lanes stay or leave together.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int32_t* abort) {
@@ -215,6 +231,14 @@ __device__ __forceinline__ void tensor_store16(uint32_t to, const uint32_t (&x)[
       "r"(to)
       : "memory");
 }
+__device__ __forceinline__ void tensor_store32(uint32_t to, const float (&x)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,"
+      "%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::
+          KVOFF_LIST16(KVOFF_IN_F, x, 0),
+      KVOFF_LIST16(KVOFF_IN_F, x, 16), "r"(to)
+      : "memory");
+}
 // Eight columns times `by`, in place.
 __device__ __forceinline__ void tensor_scale8(uint32_t at, float by) {
   float x[8];
@@ -245,22 +269,18 @@ __device__ __forceinline__ uint32_t widen(uint32_t pair) {  // two e4m3 -> f16x2
   return r;
 }
 
-// What of a segment all roles agree on.
-struct View {
-  int keys;    // that the last row sees: nothing is read behind them
-  int fewest;  // that the first row sees
-  int rows;
-  __device__ __forceinline__ View(const Args& a, const Sequence& seq, const Segment& seg) {
-    keys = min(seq.keys(a, seg.tile), seq.context);
-    fewest = max(0, seq.context - seq.q_len + seg.tile * a.rows / a.group + 1);
-    rows = min(a.rows, seq.q_len * a.group - seg.tile * a.rows);
-  }
-  __device__ __forceinline__ int groups() const { return rows > kGroupRows ? 2 : 1; }
-  // Whether rows see key tile `tile` to different lengths.
-  __device__ __forceinline__ bool mixed(int tile) const {
-    return (tile + 1) * kKeyTile > fewest && fewest < keys;
-  }
-};
+template <int kRegisters>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegisters));
+}
+template <int kRegisters>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegisters));
+}
+// 512 threads are launched with 128 registers each; the shares of the four
+// warpgroups add up to 4 * 128.
+constexpr int kSoftmaxRegisters = 152, kConvertRegisters = 112, kIssueRegisters = 96;
+static_assert(2 * kSoftmaxRegisters + kConvertRegisters + kIssueRegisters == 4 * 128, "registers");
 
 // Chunk `chunk` (8 f16 values) of row `row` of an operand.
 template <int D>
@@ -272,18 +292,6 @@ __device__ __forceinline__ void store_shared(uint32_t to, uint4 v) {
                : "memory");
 }
 
-// The warp's next segment, whose sequence is walk.seq, or false.
-__device__ __forceinline__ bool next_segment(const Args& a, Shared::Place& place, bool first) {
-  bool more = false;
-  __syncwarp();
-  if (threadIdx.x % 32 == 0) {
-    if (!first) place.walk.advance(a);
-    more = place.walk.next(a, &place.segment);
-  }
-  __syncwarp();
-  return __any_sync(0xFFFFFFFFu, more);
-}
-
 __device__ __forceinline__ uint4 load_shared(uint32_t p) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
@@ -291,6 +299,11 @@ __device__ __forceinline__ uint4 load_shared(uint32_t p) {
                : "r"(p)
                : "memory");
   return v;
+}
+// Two values of q, and of out, in a word.
+__device__ __forceinline__ float2 unpack(bool bf16, uint32_t w) {
+  if (bf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 __device__ __forceinline__ uint32_t pack_out(const Args& a, float x, float y) {
   uint32_t r;
@@ -301,56 +314,100 @@ __device__ __forceinline__ uint32_t pack_out(const Args& a, float x, float y) {
   return r;
 }
 
+// The next segment for a warp (or, in the issuing role, a thread), or null.
+__device__ __forceinline__ const Work* take_work(Shared* sh, uint32_t n) {
+  const Work* work = &sh->work[n % kWorkRing];
+  if (!bar_wait(&sh->work_full[n % kWorkRing], n / kWorkRing & 1, &sh->abort) || work->end < 0) return nullptr;
+  return work;
+}
+__device__ __forceinline__ void return_work(Shared* sh, uint32_t n) { bar_arrive(&sh->work_empty[n % kWorkRing]); }
+
+// --- warp 13 ---------------------------------------------------------------
+
+__device__ __forceinline__ void schedule_role(const Args& a, Walk<kThreads>& walk, Shared* sh) {
+  uint32_t n = 0;
+  Segment seg;
+  for (bool more = true; more; ++n) {
+    more = walk.next(a, &seg);
+    if (!bar_wait(&sh->work_empty[n % kWorkRing], (n / kWorkRing & 1) ^ 1, &sh->abort)) return;
+    Work& w = sh->work[n % kWorkRing];
+    w.end = -1;
+    if (more) {
+      const Sequence& seq = walk.seq;
+      w.begin = seg.begin, w.end = seg.end;
+      w.seq = seg.seq, w.head = seg.head;
+      w.slot = seg.whole ? -1 : seg.slot;
+      w.start = seq.start, w.offset = seq.context - seq.q_len;
+      w.first_row = seg.tile * a.rows;
+      w.rows = min(a.rows, seq.q_len * a.group - w.first_row);
+      w.keys = min(seq.keys(a, seg.tile), seq.context);
+      w.fewest = max(0, w.offset + w.first_row / a.group + 1);
+      walk.advance(a);
+    }
+    bar_arrive(&sh->work_full[n % kWorkRing]);
+  }
+  walk.finish(a);
+}
+
 // --- warps 8-11 ------------------------------------------------------------
+
+// Volatile: it stays where it stands, a key tile ahead of its use.
+__device__ __forceinline__ uint4 load_global(const uint8_t* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
 
 template <int D>
 struct Convert {
-  static constexpr int kChunks = D / 16;         // 16-byte chunks of a row
-  static constexpr int kPasses = kChunks;        // 128 threads over 128 rows
+  static constexpr int kChunks = D / 16;  // 16-byte chunks of a row
+  static constexpr int kPasses = kChunks;  // 128 threads over 128 rows
   static constexpr int kRowsAPass = 128 / kChunks;
   const Args& a;
   Shared* sh;
   uint32_t base;
   int t;  // thread of the warpgroup
 
-  // The group (16 keys) that pass i of this thread reads.
-  __device__ __forceinline__ int row(int i) const { return t / kChunks + kRowsAPass * i; }
+  // Chunk and first row of this thread. Eight threads have four chunks of an
+  // even row and of the next one, whose swizzled places in shared memory are
+  // all different.
+  __device__ __forceinline__ int chunk() const { return D == 128 ? t % 4 + t / 8 % 2 * 4 : t % 4; }
+  __device__ __forceinline__ int row0() const { return D == 128 ? t / 32 * 4 + t / 16 % 2 * 2 + t / 4 % 2 : t / 4; }
+  __device__ __forceinline__ int row(int i) const { return row0() + kRowsAPass * i; }
 
-  __device__ __forceinline__ void load(int kv, const View& view, const Segment& seg, int tile, int page_of,
-                                       uint4 (&raw)[kPasses]) const {
-    const int chunk = t % kChunks;
-    const uint8_t* cache = kv != 0 ? a.cache[1] : a.cache[0];
+  // `place`: in lane g < 8, where 16-key group g begins in the cache (bytes, at
+  // this head), or negative when it has no page. `left`: keys of the tile that
+  // are read.
+  __device__ __forceinline__ void load(int kv, int64_t place, int left, uint4 (&raw)[kPasses]) const {
     const int64_t row_bytes = (int64_t)a.kv_heads * D;
+    const uint8_t* from =
+        (kv != 0 ? a.cache[1] : a.cache[0]) + row0() % 16 * row_bytes + chunk() * 16;
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
-      const int r = row(i), key = tile * kKeyTile + r;
-      const int page = __shfl_sync(0xFFFFFFFFu, page_of, r / 16);
+      const int64_t at = __shfl_sync(0xFFFFFFFFu, place, row(i) / 16);
       raw[i] = make_uint4(0, 0, 0, 0);
-      if (key < view.keys && page >= 0)
-        raw[i] = __ldg(reinterpret_cast<const uint4*>(
-            cache + ((int64_t)page * a.page + key % a.page) * row_bytes + seg.head * D + chunk * 16));
+      if (row(i) < left && at >= 0) raw[i] = load_global(from + at);
     }
   }
 
   __device__ __forceinline__ void put(uint32_t to, const uint4 (&raw)[kPasses]) const {
-    const int chunk = t % kChunks;
+    // The swizzle is the same in all passes: they are 16 or 32 rows apart.
+    const uint32_t first = to + operand_at<D>(row0(), 2 * chunk()), second = to + operand_at<D>(row0(), 2 * chunk() + 1);
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
-      const uint4 lo = make_uint4(widen(raw[i].x & 0xFFFFu), widen(raw[i].x >> 16),
-                                  widen(raw[i].y & 0xFFFFu), widen(raw[i].y >> 16));
-      const uint4 hi = make_uint4(widen(raw[i].z & 0xFFFFu), widen(raw[i].z >> 16),
-                                  widen(raw[i].w & 0xFFFFu), widen(raw[i].w >> 16));
-      // The threads of the second block of a row write their halves in the
-      // other order: eight threads meet all banks.
-      const bool swap = chunk >= 4;
-      store_shared(to + operand_at<D>(row(i), 2 * chunk + swap), swap ? hi : lo);
-      store_shared(to + operand_at<D>(row(i), 2 * chunk + !swap), swap ? lo : hi);
+      store_shared(first + i * kRowsAPass * 128,
+                   make_uint4(widen(raw[i].x & 0xFFFFu), widen(raw[i].x >> 16),
+                              widen(raw[i].y & 0xFFFFu), widen(raw[i].y >> 16)));
+      store_shared(second + i * kRowsAPass * 128,
+                   make_uint4(widen(raw[i].z & 0xFFFFu), widen(raw[i].z >> 16),
+                              widen(raw[i].w & 0xFFFFu), widen(raw[i].w >> 16)));
     }
   }
 
   // Takes NaN out of V and notes them, one bit each, per key and chunk.
   __device__ __forceinline__ void take_nan(int stage, uint32_t count, uint4 (&raw)[kPasses], uint8_t* masks) const {
-    const int chunk = t % kChunks;
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
       uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
@@ -362,206 +419,240 @@ struct Convert {
         mask |= ((is & 1u) | (is >> 7 & 2u) | (is >> 14 & 4u) | (is >> 21 & 8u)) << 4 * k;
       }
       raw[i] = make_uint4(w[0], w[1], w[2], w[3]);
-      reinterpret_cast<uint16_t*>(masks)[row(i) * kChunks + chunk] = (uint16_t)mask;
+      reinterpret_cast<uint16_t*>(masks)[row(i) * kChunks + chunk()] = (uint16_t)mask;
       if (mask != 0) *reinterpret_cast<volatile uint32_t*>(&sh->nan[stage]) = count + 1;
     }
   }
 };
 
 template <int D>
-__device__ __forceinline__ void convert_role(const Args& a, Shared::Place& place, Shared* sh, uint8_t* smem) {
+__device__ __forceinline__ void convert_role(const Args& a, Shared* sh, uint8_t* smem) {
   Convert<D> c{a, sh, smem_of(smem), (int)threadIdx.x % 128};
   constexpr int kPasses = Convert<D>::kPasses;
   using L = Layout<D>;
   const int lane = threadIdx.x % 32;
   const int blocks = a.page / 16 / a.block_tiles;  // scale blocks of a page
   uint32_t count = 0;  // key tiles so far, over all segments
-  for (bool first = true; next_segment(a, place, first); first = false) {
-    const Segment seg = place.segment;
-    const View view(a, place.walk.seq, seg);
-    const int32_t* table = a.tables + seg.seq * a.table_stride;
-    // Lane g < 8 of each warp holds the page of group g of a tile, -1 for none.
+  for (uint32_t n = 0;; ++n) {
+    const Work* work = take_work(sh, n);
+    if (__any_sync(0xFFFFFFFFu, work == nullptr)) return;
+    const int32_t* table = a.tables + work->seq * a.table_stride;
+    const int begin = work->begin, end = work->end, keys = work->keys, head = work->head;
+    // Lane g < 8 of each warp has the page of group g of a tile (checked when it
+    // is used, a tile later), and from it where the group's rows and scales begin.
     auto page_of = [&](int tile) {
       const int key = tile * kKeyTile + lane * 16;
-      int id = -1;
-      if (lane < 8 && tile < seg.end && key < view.keys) {
-        id = __ldg(table + key / a.page);
-        if (id >= a.num_pages) id = -1;
-      }
-      return id < 0 ? -1 : id;
+      return lane < 8 && tile < end && key < keys ? __ldg(table + key / a.page) : -1;
     };
-    float k_scale = 0.0f, v_scale = 0.0f;
+    int page_next = page_of(begin);
+    int64_t place = -1;
+    float k_scale = 0.0f, v_scale = 0.0f, largest = -200.0f;
     uint32_t absent = 0;
-    auto load_scales = [&](int tile, int page) {
-      k_scale = v_scale = 0.0f;
-      const int key = tile * kKeyTile + lane * 16;
-      if (page >= 0) {
-        const int64_t at =
-            ((int64_t)page * blocks + key % a.page / 16 / a.block_tiles) * a.kv_heads + seg.head;
-        k_scale = __ldg(a.scale[0] + at);
-        v_scale = __ldg(a.scale[1] + at);
-      }
-      absent = __ballot_sync(0xFFFFFFFFu, page < 0) & 0xFFu;
-    };
     uint4 k_raw[kPasses], v_raw[kPasses];
-    int page = page_of(seg.begin), page_next = page_of(seg.begin + 1);
-    c.load(0, view, seg, seg.begin, page, k_raw);
-    c.load(1, view, seg, seg.begin, page, v_raw);
-    load_scales(seg.begin, page);
-    for (int tile = seg.begin; tile < seg.end; ++tile, ++count) {
-      const int stage = count % kStages;
-      const uint32_t parity = (count / kStages & 1) ^ 1;
-      if (!warp_wait(&sh->k_empty[stage], parity, &sh->abort)) return;
-      c.put(c.base + L::kK + stage * L::kOperand, k_raw);
-      if (c.t < 32) {
-        Scales& s = sh->scales[count % kScaleRing];
-        if (lane < 8) {
-          s.k[lane] = k_scale;
-          s.v_log2[lane] = v_scale > 0.0f ? log2f(v_scale) : v_scale == v_scale ? -200.0f : v_scale;
+    // Tile `tile` is put into shared memory while tile + 1 is loaded.
+#pragma unroll 1
+    for (int tile = begin - 1; tile < end; ++tile) {
+      if (tile >= begin) {
+        const int stage = count % kStages;
+        const uint32_t parity = (count / kStages & 1) ^ 1;
+        if (!warp_wait(&sh->k_empty[stage], parity, &sh->abort)) return;
+        c.put(c.base + L::kK + stage * L::kOperand, k_raw);
+        if (c.t < 32) {
+          Scales& s = sh->scales[count % kScaleRing];
+          const float log2 = v_scale > 0.0f ? log2f(v_scale) : v_scale == v_scale ? -200.0f : v_scale;
+          float most = lane < 8 ? log2 : -200.0f;
+#pragma unroll
+          for (int d = 4; d > 0; d /= 2) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
+          largest = fmaxf(largest, __shfl_sync(0xFFFFFFFFu, most, 0));
+          if (lane < 8) {
+            const float relative = log2 - largest;
+            const float shift = (relative < kLeastLog2 ? kLeastLog2 : relative) + kWeightLog2;
+            s.k[lane] = k_scale;
+            s.shift[lane] = shift;
+            s.inverse[lane] = exp2_fast(-shift);
+          }
+          if (lane == 0) {
+            s.largest = largest;
+            s.absent = absent;
+          }
+          __syncwarp();
+          if (lane == 0) bar_arrive(&sh->scale_full[count % kScaleRing]);
         }
-        if (lane == 0) s.absent = absent;
-        __syncwarp();
-        if (lane == 0) bar_arrive(&sh->scale_full[count % kScaleRing]);
+        async_fence();
+        bar_arrive(&sh->k_full[stage]);
+        if (!warp_wait(&sh->v_empty[stage], parity, &sh->abort)) return;
+        if (work->mixed(tile)) c.take_nan(stage, count, v_raw, smem + L::kNan + stage * L::kNanBytes);
+        c.put(c.base + L::kV + stage * L::kOperand, v_raw);
+        async_fence();
+        bar_arrive(&sh->v_full[stage]);
+        ++count;
       }
-      async_fence();
-      bar_arrive(&sh->k_full[stage]);
-      const bool more = tile + 1 < seg.end;
-      page = page_next;
-      if (more) {
+      if (tile + 1 < end) {
+        const int page = page_next < a.num_pages ? page_next : -1;
         page_next = page_of(tile + 2);
-        c.load(0, view, seg, tile + 1, page, k_raw);
-        load_scales(tile + 1, page);
+        place = -1;
+        k_scale = v_scale = 0.0f;
+        if (page >= 0) {
+          const int in_page = ((tile + 1) * kKeyTile + lane * 16) % a.page;
+          place = ((int64_t)page * a.page + in_page) * a.kv_heads * D + head * D;
+          const int64_t at = ((int64_t)page * blocks + in_page / 16 / a.block_tiles) * a.kv_heads + head;
+          k_scale = __ldg(a.scale[0] + at);
+          v_scale = __ldg(a.scale[1] + at);
+        }
+        absent = __ballot_sync(0xFFFFFFFFu, page < 0) & 0xFFu;
+        c.load(0, place, keys - (tile + 1) * kKeyTile, k_raw);
+        c.load(1, place, keys - (tile + 1) * kKeyTile, v_raw);
       }
-      if (!warp_wait(&sh->v_empty[stage], parity, &sh->abort)) return;
-      if (view.mixed(tile)) {
-        c.take_nan(stage, count, v_raw, smem + L::kNan + stage * L::kNanBytes);
-      }
-      c.put(c.base + L::kV + stage * L::kOperand, v_raw);
-      async_fence();
-      bar_arrive(&sh->v_full[stage]);
-      if (more) c.load(1, view, seg, tile + 1, page, v_raw);
     }
+    __syncwarp();
+    if (lane == 0) return_work(sh, n);
   }
 }
 
 // --- warp 12 ---------------------------------------------------------------
 
 template <int D>
-__device__ __forceinline__ void issue_role(const Args& a, Shared::Place& place, Shared* sh, uint32_t base) {
+__device__ __forceinline__ void issue_role(Shared* sh, uint32_t base) {
   using L = Layout<D>;
   const uint32_t tmem = sh->tmem;
-  uint32_t count = 0, turn[2] = {0, 0}, segment[2] = {0, 0};
-  auto scores = [&](int g, int stage) {
-#pragma unroll
-    for (int k = 0; k < D / 16; ++k) {
-      const uint32_t at = (k / 4) * 16384 + (k % 4) * 32;
-      mma_shared(tmem + kScoresAt + g * kGroupColumns, row_descriptor(base + L::kQ + g * L::kOperand + at),
-                 row_descriptor(base + L::kK + stage * L::kOperand + at), kInstruction<128, false>, k > 0);
-    }
-    commit(&sh->s_full[g]);
-  };
-  for (; place.walk.next(a, &place.segment); place.walk.advance(a)) {
-    const Segment seg = place.segment;
-    const View view(a, place.walk.seq, seg);
-    const int groups = view.groups(), tiles = seg.end - seg.begin;
-    if (!bar_wait(&sh->k_full[count % kStages], count / kStages & 1, &sh->abort)) return;
-    for (int g = 0; g < groups; ++g) {
-      if (!bar_wait(&sh->q_full[g], segment[g] & 1, &sh->abort)) return;
-      ++segment[g];
-      tensor_fence_after();
-      scores(g, count % kStages);
-    }
-    commit(&sh->k_empty[count % kStages]);
-    for (int i = 0; i < tiles; ++i, ++count) {
-      const int stage = count % kStages, next = (count + 1) % kStages;
-      if (!bar_wait(&sh->v_full[stage], count / kStages & 1, &sh->abort)) return;
+  uint32_t count = 0;                // key tiles so far
+  uint32_t turn[2] = {0, 0}, segment[2] = {0, 0};
+  for (uint32_t n = 0;; ++n) {
+    const Work* work = take_work(sh, n);
+    if (work == nullptr) return;
+    const int groups = work->groups(), tiles = work->end - work->begin;
+    return_work(sh, n);
+    // Step i: the output of key tile i - 1, then the scores of tile i.
+#pragma unroll 1
+    for (int i = 0; i <= tiles; ++i) {
+      const uint32_t now = count + i, before = now - 1;
+#pragma unroll 1
       for (int g = 0; g < groups; ++g) {
-        if (!bar_wait(&sh->p_full[g], turn[g] & 1, &sh->abort)) return;
-        ++turn[g];
-        tensor_fence_after();
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          mma_tensor(tmem + kOutputsAt + g * kGroupColumns, tmem + kScoresAt + g * kGroupColumns + k * 8,
-                     column_descriptor(base + L::kV + stage * L::kOperand + k * 2048), kInstruction<D, true>,
-                     i > 0 || k > 0);
-        if (g == groups - 1) commit(&sh->v_empty[stage]);
-        if (i + 1 < tiles) {
-          if (g == 0 && !bar_wait(&sh->k_full[next], (count + 1) / kStages & 1, &sh->abort)) return;
+        const uint32_t scores = tmem + kScoresAt + g * kGroupColumns, output = tmem + kOutputsAt + g * kGroupColumns;
+        if (i > 0) {
+          if (!bar_wait(&sh->v_full[before % kStages], before / kStages & 1, &sh->abort)) return;
+          uint32_t& t = g == 0 ? turn[0] : turn[1];
+          if (!bar_wait(&sh->p_full[g], t & 1, &sh->abort)) return;
+          ++t;
           tensor_fence_after();
-          scores(g, next);
-          if (g == groups - 1) commit(&sh->k_empty[next]);
-        } else {
-          commit(&sh->o_full[g]);
+          const uint64_t v = column_descriptor(base + L::kV + before % kStages * L::kOperand);
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            mma_tensor(output, scores + k * 8, v + (k * 2048 >> 4), kInstruction<D, true>, i > 1 || k > 0);
+          if (g == groups - 1) commit(&sh->v_empty[before % kStages]);
+          if (i == tiles) commit(&sh->o_full[g]);
+        }
+        if (i < tiles) {
+          if (!bar_wait(&sh->k_full[now % kStages], now / kStages & 1, &sh->abort)) return;
+          if (i == 0) {
+            uint32_t& t = g == 0 ? segment[0] : segment[1];
+            if (!bar_wait(&sh->q_full[g], t & 1, &sh->abort)) return;
+            ++t;
+          }
+          tensor_fence_after();
+          const uint64_t q = row_descriptor(base + L::kQ + g * L::kOperand);
+          const uint64_t keys = row_descriptor(base + L::kK + now % kStages * L::kOperand);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t at = ((k / 4) * 16384 + (k % 4) * 32) >> 4;
+            mma_shared(scores, q + at, keys + at, kInstruction<128, false>, k > 0);
+          }
+          commit(&sh->s_full[g]);
+          if (g == groups - 1) commit(&sh->k_empty[now % kStages]);
         }
       }
     }
+    count += tiles;
   }
 }
 
 // --- warps 0-7 -------------------------------------------------------------
 
+// Scores behind the row's last key, or of groups without a page, become -inf.
+__device__ __forceinline__ void mask_scores(uint32_t scores_at, int seen, uint32_t absent) {
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    float s[32];
+    load_begin(s, scores_at + 32 * c);
+    load_end(s);
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (32 * c + i >= seen || (absent >> (2 * c + i / 16) & 1)) s[i] = __uint_as_float(kNegInf);
+    tensor_store32(scores_at + 32 * c, s);
+  }
+  tensor_wait_stores();
+}
+
+// Two at a time: the fp32 pairs of sm_100 take one issue slot.
+__device__ __forceinline__ float2 exp2_pair(float x, float y, float f, float bias) {
+  uint64_t r;
+  asm("{\n\t.reg .b64 x, f, b;\n\tmov.b64 x, {%1, %2};\n\tmov.b64 f, {%3, %3};\n\tmov.b64 b, {%4, %4};\n\t"
+      "fma.rn.f32x2 %0, x, f, b;\n\t}"
+      : "=l"(r)
+      : "f"(x), "f"(y), "f"(f), "f"(bias));
+  return make_float2(exp2_fast(__uint_as_float((uint32_t)r)), exp2_fast(__uint_as_float((uint32_t)(r >> 32))));
+}
+__device__ __forceinline__ float2 add_pair(float2 a, float2 b) {
+  uint64_t r;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%1, %2};\n\tmov.b64 y, {%3, %4};\n\tadd.rn.f32x2 %0, x, y;\n\t}"
+      : "=l"(r)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return make_float2(__uint_as_float((uint32_t)r), __uint_as_float((uint32_t)(r >> 32)));
+}
+
+// --- warps 0-7 -------------------------------------------------------------
+
 template <int D>
-__device__ __forceinline__ void softmax_role(const Args& a, Shared::Place& place, Shared* sh, uint8_t* smem) {
+__device__ __forceinline__ void softmax_role(const Args& a, Shared* sh, uint8_t* smem) {
   using L = Layout<D>;
   const int g = threadIdx.x / 128, r = threadIdx.x % 128;
   const uint32_t base = smem_of(smem);
   const uint32_t lanes = (uint32_t)(r / 32 * 32) << 16;
   const uint32_t scores_at = sh->tmem + lanes + kScoresAt + g * kGroupColumns;
   const uint32_t output_at = sh->tmem + lanes + kOutputsAt + g * kGroupColumns;
+  const uint32_t q_at = base + L::kQ + g * L::kOperand;
   uint32_t count = 0, turn = 0, segment = 0;
-  for (bool first = true; next_segment(a, place, first); first = false) {
-    const Sequence& seq = place.walk.seq;
-    const Segment& seg = place.segment;
-    const View view(a, seq, seg);
-    if (g >= view.groups()) {
-      count += seg.end - seg.begin;
+  for (uint32_t n = 0;; ++n) {
+    const Work* work = take_work(sh, n);
+    if (__any_sync(0xFFFFFFFFu, work == nullptr)) return;
+    const int begin = work->begin, end = work->end;
+    if (g >= work->groups()) {
+      count += end - begin;
+      __syncwarp();
+      if (threadIdx.x % 32 == 0) return_work(sh, n);
       continue;
     }
-    const int at = seg.tile * a.rows + g * kGroupRows + r;  // this thread's packed row
-    const bool real = g * kGroupRows + r < view.rows;
-    const int token = seq.start + at / a.group, head = seg.head * a.group + at % a.group;
-    const int limit = real ? max(0, seq.context - seq.q_len + at / a.group + 1) : 0;
+    const int at = work->first_row + g * kGroupRows + r;  // this thread's packed row
+    const bool real = g * kGroupRows + r < work->rows;
+    const int limit = real ? max(0, work->offset + at / a.group + 1) : 0;  // keys that it sees
     float factor;
     {  // q: one row a thread, scaled to an amax of 2^14..2^15
-      const uint4* from =
-          reinterpret_cast<const uint4*>(a.q + token * a.q_stride + (int64_t)head * D * 2);
-      uint32_t most = 0;
-      auto values = [&](const uint4& v, float (&x)[8]) {
+      const uint8_t* from = a.q + (work->start + at / a.group) * a.q_stride +
+                            (int64_t)(work->head * a.group + at % a.group) * D * 2;
+      const uint32_t infinite = a.bf16 ? 0x7F80u : 0x7C00u;
+      uint32_t most = 0;  // magnitude bits of the largest finite value
+#pragma unroll 4
+      for (int c = 0; c < D / 8; ++c) {
+        const uint4 v = real ? __ldg(reinterpret_cast<const uint4*>(from) + c) : make_uint4(0, 0, 0, 0);
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float2 f;
-          if (a.bf16)
-            f = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
-          else
-            f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-          x[2 * i] = f.x, x[2 * i + 1] = f.y;
-        }
-      };
-      uint4 raw[D / 8];
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c) raw[c] = real ? __ldg(from + c) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        float x[8];
-        values(raw[c], x);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t u = __float_as_uint(x[i]) & 0x7FFFFFFFu;
-          if (u < 0x7F800000u) most = max(most, u);
+          const uint32_t lo = w[i] & 0x7FFFu, hi = w[i] >> 16 & 0x7FFFu;
+          most = max(most, max(lo < infinite ? lo : 0u, hi < infinite ? hi : 0u));
         }
       }
-      const int e = most == 0 ? 0 : min(14 - ((int)(most >> 23) - 127), 100);
+      const uint32_t bits = __float_as_uint(unpack(a.bf16, most).x);
+      const int e = bits == 0 ? 0 : min(14 - ((int)(bits >> 23) - 127), 100);
       const float up = __uint_as_float((uint32_t)(127 + e) << 23);
       factor = a.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23);
-      const uint32_t to = base + L::kQ + g * L::kOperand;
-#pragma unroll
+#pragma unroll 4
       for (int c = 0; c < D / 8; ++c) {
-        float x[8];
-        values(raw[c], x);
-        store_shared(to + operand_at<D>(r, c),
-                     make_uint4(pack_half(x[0] * up, x[1] * up), pack_half(x[2] * up, x[3] * up),
-                                pack_half(x[4] * up, x[5] * up), pack_half(x[6] * up, x[7] * up)));
+        const uint4 v = real ? __ldg(reinterpret_cast<const uint4*>(from) + c) : make_uint4(0, 0, 0, 0);
+        const float2 x0 = unpack(a.bf16, v.x), x1 = unpack(a.bf16, v.y);
+        const float2 x2 = unpack(a.bf16, v.z), x3 = unpack(a.bf16, v.w);
+        store_shared(q_at + operand_at<D>(r, c),
+                     make_uint4(pack_half(x0.x * up, x0.y * up), pack_half(x1.x * up, x1.y * up),
+                                pack_half(x2.x * up, x2.y * up), pack_half(x3.x * up, x3.y * up)));
       }
       async_fence();
       tensor_fence_before();
@@ -572,91 +663,82 @@ __device__ __forceinline__ void softmax_role(const Args& a, Shared::Place& place
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) nan[i] = 0;
 
-    for (int tile = seg.begin; tile < seg.end; ++tile, ++count) {
-      if (!warp_wait(&sh->s_full[g], turn & 1, &sh->abort)) return;
-      ++turn;
-      tensor_fence_after();
-      const Scales& scales = sh->scales[count % kScaleRing];
+#pragma unroll 1
+    for (int tile = begin; tile < end; ++tile, ++count) {
       if (!warp_wait(&sh->scale_full[count % kScaleRing], count / kScaleRing & 1, &sh->abort)) return;
+      const Scales& scales = sh->scales[count % kScaleRing];
+      float f[8];
+#pragma unroll
+      for (int b = 0; b < 8; ++b)  // a scale of zero must not meet a masked score's infinity
+        f[b] = fmaxf(scales.k[b] * factor, 1e-37f);
+      const float largest = scales.largest;
       const uint32_t absent = scales.absent;
       const int seen = limit - tile * kKeyTile;  // of this tile's keys
       const bool masked = __any_sync(0xFFFFFFFFu, seen < kKeyTile) || absent != 0;
-      auto mask = [&](int c, float (&s)[32]) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (32 * c + i >= seen || (absent >> (2 * c + i / 16) & 1)) s[i] = __uint_as_float(kNegInf);
-      };
-      // A scale of zero must not meet a masked score's infinity.
-      auto factor_of = [&](int b) { return fmaxf(scales.k[b] * factor, 1e-37f); };
+      if (!warp_wait(&sh->s_full[g], turn & 1, &sh->abort)) return;
+      ++turn;
+      tensor_fence_after();
+      if (masked) mask_scores(scores_at, seen, absent);
 
       // The row's maximum; then its scores again, which costs less than the
       // registers to keep them.
       float buffer[2][32];
-      float most = __uint_as_float(kNegInf), ref_now = ref;
+      float most = __uint_as_float(kNegInf);
       load_begin(buffer[0], scores_at);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         float(&s)[32] = buffer[c % 2];
         load_end(s);
         load_begin(buffer[(c + 1) % 2], scores_at + (c + 1) % 4 * 32);
-        if (masked) mask(c, s);
+        float top[4] = {s[0], s[1], s[16], s[17]};
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          float top = s[16 * b];
-#pragma unroll
-          for (int i = 1; i < 16; ++i) top = fmaxf(top, s[16 * b + i]);
-          most = fmaxf(most, top * factor_of(2 * c + b));
-          ref_now = fmaxf(ref_now, scales.v_log2[2 * c + b]);
+        for (int i = 2; i < 16; i += 2) {
+          top[0] = fmaxf(top[0], s[i]), top[1] = fmaxf(top[1], s[i + 1]);
+          top[2] = fmaxf(top[2], s[16 + i]), top[3] = fmaxf(top[3], s[17 + i]);
         }
+        most = fmaxf(most, fmaxf(fmaxf(top[0], top[1]) * f[2 * c], fmaxf(top[2], top[3]) * f[2 * c + 1]));
       }
       load_end(buffer[0]);
-      if (__any_sync(0xFFFFFFFFu, most > m + kRaise || ref_now > ref)) {
+      if (__any_sync(0xFFFFFFFFu, most > m + kRaise || largest > ref)) {
         const float top = fmaxf(m, most);
         const float keep_l = top == m ? 1.0f : exp2_fast(m - top);
-        if (tile != seg.begin) {
-          const float keep = keep_l * exp2_fast(ref - ref_now);
+        if (tile != begin) {
+          const float keep = keep_l * exp2_fast(ref - largest);
 #pragma unroll 1
           for (int c = 0; c < D / 8; ++c) tensor_scale8(output_at + 8 * c, keep);
         }
         l *= keep_l;
         m = top;
-        ref = ref_now;
+        ref = largest;
       }
       const float shift = m == __uint_as_float(kNegInf) ? 0.0f : m;
-      float scale_log2 = 0.0f, last = 1e30f, unscale = 1.0f;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         float(&s)[32] = buffer[c % 2];
         if (c > 0) load_end(s);
         if (c < 3) load_begin(buffer[(c + 1) % 2], scores_at + (c + 1) * 32);
-        if (masked) mask(c, s);
         uint32_t p[16];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int b = 2 * c + k;
-          const float v_log2 = scales.v_log2[b];
-          if (v_log2 != last) {  // one number for all of a larger scale block
-            last = v_log2;
-            const float relative = v_log2 - ref;
-            scale_log2 = (relative < kLeastLog2 ? kLeastLog2 : relative) + kWeightLog2;
-            unscale = exp2_fast(-scale_log2);
-          }
-          const float f = factor_of(b), bias = scale_log2 - shift;
-          float sum0 = 0.0f, sum1 = 0.0f;
+          const float bias = scales.shift[b] - shift;
+          float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0;
 #pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            const float x = exp2_fast(fmaf(s[16 * k + i], f, bias));
-            const float y = exp2_fast(fmaf(s[16 * k + i + 1], f, bias));
-            sum0 += x;
-            sum1 += y;
-            p[8 * k + i / 2] = pack_half(x, y);
+          for (int i = 0; i < 16; i += 4) {
+            const float2 x = exp2_pair(s[16 * k + i], s[16 * k + i + 1], f[b], bias);
+            const float2 y = exp2_pair(s[16 * k + i + 2], s[16 * k + i + 3], f[b], bias);
+            sum0 = add_pair(sum0, x);
+            sum1 = add_pair(sum1, y);
+            p[8 * k + i / 2] = pack_half(x.x, x.y);
+            p[8 * k + i / 2 + 1] = pack_half(y.x, y.y);
           }
-          l = fmaf(sum0 + sum1, unscale, l);
+          sum0 = add_pair(sum0, sum1);
+          l = fmaf(sum0.x + sum0.y, scales.inverse[b], l);
         }
         // P takes the columns of scores that have been read: 16 for these 32.
         tensor_store16(scores_at + 16 * c, p);
       }
-      if (view.mixed(tile)) {
+      if (work->mixed(tile)) {
         const int stage = count % kStages;
         if (!warp_wait(&sh->v_full[stage], count / kStages & 1, &sh->abort)) return;
         if (*reinterpret_cast<volatile uint32_t*>(&sh->nan[stage]) == count + 1) {
@@ -676,10 +758,10 @@ __device__ __forceinline__ void softmax_role(const Args& a, Shared::Place& place
     ++segment;
     tensor_fence_after();
     // exp2(ref) may be as small as a scale can be; a row of zero scales is zero.
-    const float scale = exp2_fast(ref - kWeightLog2) * (seg.whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f);
-    float* slot = seg.whole ? nullptr : a.partial + ((int64_t)place.walk.cta * 2 + seg.slot) * slot_floats(a.rows, D);
+    const bool whole = work->slot < 0;
+    const float scale = exp2_fast(ref - kWeightLog2) * (whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f);
+    float* slot = whole ? nullptr : a.partial + ((int64_t)blockIdx.x * 2 + work->slot) * slot_floats(a.rows, D);
     const int row = g * kGroupRows + r;
-    const uint32_t stage_at = base + L::kQ + g * L::kOperand;  // q is not read any more
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
       float o[32];
@@ -688,16 +770,12 @@ __device__ __forceinline__ void softmax_role(const Args& a, Shared::Place& place
       load_end(o);
 #pragma unroll
       for (int i = 0; i < 32; ++i) o[i] = (nan[c] >> i & 1) != 0 ? __uint_as_float(0x7FC00000u) : o[i] * scale;
-      if (seg.whole && a.wide_out) {
+      if (whole) {  // through the tile of q, which is not read any more
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          store_shared(stage_at + operand_at<D>(r, 4 * c + k),
+          store_shared(q_at + operand_at<D>(r, 4 * c + k),
                        make_uint4(pack_out(a, o[8 * k], o[8 * k + 1]), pack_out(a, o[8 * k + 2], o[8 * k + 3]),
                                   pack_out(a, o[8 * k + 4], o[8 * k + 5]), pack_out(a, o[8 * k + 6], o[8 * k + 7])));
-      } else if (seg.whole) {
-        if (real)
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) write_pair(a, token, head, D, 32 * c + i, o[i], o[i + 1]);
       } else if (real) {
         float4* to = reinterpret_cast<float4*>(slot + (int64_t)row * D + 32 * c);
 #pragma unroll
@@ -706,25 +784,31 @@ __device__ __forceinline__ void softmax_role(const Args& a, Shared::Place& place
       }
     }
     __syncwarp();
-    if (seg.whole && a.wide_out) {  // the warp's 32 rows, D / 8 threads to a row
+    if (whole) {  // the warp's 32 rows, D / 8 threads to a row
       const int first_row = g * kGroupRows + r / 32 * 32;
-#pragma unroll 4
+#pragma unroll 2
       for (int i = threadIdx.x % 32; i < 32 * (D / 8); i += 32) {
         const int k = i / (D / 8), chunk = i % (D / 8);
-        if (first_row + k < view.rows) {
-          const int to = seg.tile * a.rows + first_row + k;
-          uint8_t* out = a.out + (seq.start + to / a.group) * a.out_stride +
-                         (int64_t)(seg.head * a.group + to % a.group) * D * 2 + chunk * 16;
-          *reinterpret_cast<uint4*>(out) = load_shared(stage_at + operand_at<D>(r / 32 * 32 + k, chunk));
+        if (first_row + k < work->rows) {
+          const int to = work->first_row + first_row + k;
+          uint8_t* out = a.out + (work->start + to / a.group) * a.out_stride +
+                         (int64_t)(work->head * a.group + to % a.group) * D * 2 + chunk * 16;
+          const uint4 v = load_shared(q_at + operand_at<D>(r / 32 * 32 + k, chunk));
+          if (a.wide_out) {
+            *reinterpret_cast<uint4*>(out) = v;
+          } else {
+            reinterpret_cast<uint32_t*>(out)[0] = v.x, reinterpret_cast<uint32_t*>(out)[1] = v.y;
+            reinterpret_cast<uint32_t*>(out)[2] = v.z, reinterpret_cast<uint32_t*>(out)[3] = v.w;
+          }
         }
       }
-    }
-    if (real && seg.whole) write_lse(a, token, head, m, l);
-    if (real && !seg.whole) {
+      if (real) write_lse(a, work->start + at / a.group, work->head * a.group + at % a.group, m, l);
+    } else if (real) {
       slot[(int64_t)a.rows * D + row] = m;
       slot[(int64_t)a.rows * D + a.rows + row] = l;
     }
     __syncwarp();
+    if (threadIdx.x % 32 == 0) return_work(sh, n);
   }
 }
 
@@ -748,6 +832,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_extend_fp8_kernel(const
       bar_init(&sh.v_empty[i], 1);
     }
     for (int i = 0; i < kScaleRing; ++i) bar_init(&sh.scale_full[i], 1);
+    for (int i = 0; i < kWorkRing; ++i) {
+      bar_init(&sh.work_full[i], 1);
+      bar_init(&sh.work_empty[i], 13);  // warps 0-11 and the issuing thread
+    }
     bar_init(&sh.drained, 1);
     sh.abort = 0;
     sh.nan[0] = sh.nan[1] = 0;
@@ -759,27 +847,28 @@ __global__ void __launch_bounds__(kThreads, 1) attention_extend_fp8_kernel(const
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
-  {
-    const Walk<kThreads> walk(a, &sh.walk);
-    if (threadIdx.x % 32 == 0) sh.place[warp].walk = walk;
-  }
+  Walk<kThreads> walk(a, &sh.walk);
   tensor_fence_before();
   __syncthreads();
   tensor_fence_after();
 
   if (warp < 8) {
-    softmax_role<D>(a, sh.place[warp], &sh, smem);
-    if (threadIdx.x == 0) sh.place[0].walk.finish(a);
+    more_registers<kSoftmaxRegisters>();
+    softmax_role<D>(a, &sh, smem);
   } else if (warp < 12) {
-    convert_role<D>(a, sh.place[warp], &sh, smem);
+    fewer_registers<kConvertRegisters>();
+    convert_role<D>(a, &sh, smem);
   } else {
+    fewer_registers<kIssueRegisters>();
     if (threadIdx.x == 12 * 32) {
-      issue_role<D>(a, sh.place[warp], &sh, smem_of(smem));
+      issue_role<D>(&sh, smem_of(smem));
       // Nothing of this CTA's is in flight when its tensor memory is freed.
       commit(&sh.drained);
       bool done = bar_try(&sh.drained, 0);
       for (int spins = 0; !done && spins < 1 << 20; ++spins) done = bar_try(&sh.drained, 0);
       if (!done) atomicOr(&g_extend_error, kErrExtendWaitTimeout);
+    } else if (threadIdx.x == 13 * 32) {
+      schedule_role(a, walk, &sh);
     }
     __syncwarp();
   }
