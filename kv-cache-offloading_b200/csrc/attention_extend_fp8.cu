@@ -10,9 +10,11 @@
 // and each key tile is converted once for both.
 //
 //   warps 0-3, 4-7  softmax of row tile 0 and 1, one row a thread
-//   warps 8-11      cache -> registers -> f16 operands in shared memory
-//   warp 12         one thread issues all matrix products
-//   warp 13         one thread walks the CTA's part of the work
+//   warps 8-11      K: cache -> registers -> f16 operand in shared memory
+//   warps 12-15     V, in the same way
+//   warps 16, 17    one thread issues the matrix products of row tile 0, of 1
+//   warp 18         one thread walks the CTA's part of the work
+//   warp 19         pages and scales of each key tile
 //
 // K, V and Q are f16 operands: e4m3 is a subset of f16, and q is scaled by a
 // power of two to an amax of 2^14..2^15, where every bf16 value down to 2^-31
@@ -25,9 +27,9 @@
 // factor. The maximum is raised only when a score passes it by 2^6, so the
 // accumulator is rescaled a few times in a row tile, not once in each key tile.
 //
-// Order: s_full (scores of tile j) implies that all products issued before
-// them are complete, O of tile j - 1 among them, so a softmax thread may
-// rescale its row of O at any time before it reports P.
+// Scores are made 64 keys at a time, in two sets of columns that take turns: the
+// scores of half h + 1 are there when the softmax has done half h, so it does not
+// wait for products. Rescaling O waits for the output of the half before.
 //
 // Every wait is bounded; one that runs out sets an error flag that
 // kvoff_device_error reads, and all roles leave.
@@ -41,10 +43,10 @@ __device__ int g_extend_error = 0;
 
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 640;
 constexpr int kGroupRows = 128;    // rows of a tensor tile
 constexpr int kStages = 2;         // of K and of V
-constexpr int kScaleRing = 4;      // scales live longer than K's stage
+constexpr int kTileRing = 4;       // pages and scales of a tile, ahead of K and V
 constexpr int kWorkRing = 2;       // segments handed out ahead
 constexpr float kRaise = 6.0f;     // log2 of how far P may pass 1
 constexpr float kWeightLog2 = 8.0f;
@@ -53,6 +55,7 @@ constexpr uint32_t kNegInf = 0xFF800000u;
 constexpr uint32_t kWaitNs = 1000, kMostWaits = 1u << 20;  // a second in all
 constexpr uint32_t kTmemColumns = 512;
 constexpr uint32_t kScoresAt = 0, kOutputsAt = 256, kGroupColumns = 128;
+constexpr int kHalf = 64;           // keys of a step: half a key tile, half a row tile's columns
 
 template <int D>
 struct Layout {
@@ -65,15 +68,18 @@ struct Layout {
   static constexpr int kBytes = kNan + kStages * kNanBytes + 1024;  // 1024: alignment
 };
 
-// Of a tile's 16-key groups. The scale of V is a fraction of the largest one
-// that the segment has met, times 2^8: it is added to the exponent of P, and
-// its inverse takes it out of the sum of p again.
-struct Scales {
+// A key tile's 16-key groups: where they are and their scales. The scale of V
+// is a fraction of the largest one that the segment has met, times 2^8: it is
+// added to the exponent of P, and its inverse takes it out of the sum of p again.
+struct Tile {
+  int64_t place[8];  // byte of the cache, at this head; negative: no page
   float k[8];
   float shift[8];    // log2
   float inverse[8];
   float largest;     // log2 of the largest scale of V so far
   uint32_t absent;   // bit g: group g has no page
+  int32_t run;       // all 128 keys are read and follow one another from place[0]
+  int32_t pad;
 };
 
 // One segment, as the roles need it.
@@ -96,14 +102,14 @@ struct Work {
 };
 
 struct Shared {
-  uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+  uint64_t q_full[2];
+  uint64_t s_full[2][2], p_full[2][2], o_done[2][2];  // of row tile and half
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-  uint64_t scale_full[kScaleRing];
-  uint64_t drained;
-  Scales scales[kScaleRing];
+  uint64_t tile_full[kTileRing];
+  uint64_t drained[2];
+  Tile tiles[kTileRing];
   uint32_t nan[kStages];  // n + 1: V of tile n, in this stage, holds NaN that some row must not meet
   uint32_t tmem;
-  int32_t abort;
   uint64_t work_full[kWorkRing], work_empty[kWorkRing];
   Work work[kWorkRing];
   Walk<kThreads>::Shared walk;
@@ -119,34 +125,35 @@ __device__ __forceinline__ void bar_init(uint64_t* bar, uint32_t count) {
 __device__ __forceinline__ void bar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_of(bar)) : "memory");
 }
-__device__ __forceinline__ bool bar_try(uint64_t* bar, uint32_t parity) {
+// One arrival for a warp, after what all its lanes did: 128 of them would take
+// their turns at the barrier.
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+  __syncwarp();
+  if (threadIdx.x % 32 == 0) bar_arrive(bar);
+}
+// Waits for the phase of `parity`, at most kMostWaits times kWaitNs. False: the
+// error flag is set and the role leaves, after which the others run out too.
+__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\tmov.u32 n, 0;\n"
+      "AGAIN:\n\t"
       "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "@p bra DONE;\n\t"
+      "add.u32 n, n, 1;\n\t"
+      "setp.lt.u32 q, n, %4;\n\t"
+      "@q bra AGAIN;\n"
+      "DONE:\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(done)
-      : "r"(smem_of(bar)), "r"(parity), "r"(kWaitNs)
+      : "r"(smem_of(bar)), "r"(parity), "r"(kWaitNs), "n"(kMostWaits)
       : "memory");
+  if (done == 0) atomicOr(&g_extend_error, kErrExtendWaitTimeout);
   return done != 0;
 }
-
-// Waits for the phase of `parity`, at most kMostWaits times kWaitNs and not
-// once another role has given up. False: leave.
-__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, int32_t* abort) {
-  for (uint32_t i = 0; !bar_try(bar, parity); ++i) {
-    if (*reinterpret_cast<volatile int32_t*>(abort) != 0) return false;
-    if (i >= kMostWaits) {
-      *reinterpret_cast<volatile int32_t*>(abort) = 1;
-      atomicOr(&g_extend_error, kErrExtendWaitTimeout);
-      return false;
-    }
-  }
-  return true;
-}
 // The same for a whole warp, whose lanes stay or leave together.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int32_t* abort) {
-  return __all_sync(0xFFFFFFFFu, bar_wait(bar, parity, abort));
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xFFFFFFFFu, bar_wait(bar, parity));
 }
 
 __device__ __forceinline__ void tensor_fence_before() {
@@ -167,17 +174,15 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
 // Operands in shared memory: blocks of 64 f16 columns (128 bytes), 16-byte
 // chunk c of row r at chunk c ^ (r % 8), rows 128 bytes apart; blocks follow
 // one another 128 rows apart.
-constexpr uint64_t kDescriptor = (uint64_t)1 << 46      // version
-                                 | (uint64_t)2 << 61    // 128-byte swizzle
-                                 | (uint64_t)(1024 >> 4) << 32;  // from 8 rows to the next 8
-// K-major (the reduction runs along a row): the leading offset is not used.
-__device__ __forceinline__ uint64_t row_descriptor(uint32_t address) {
-  return kDescriptor | (uint64_t)1 << 16 | address >> 4;
-}
-// MN-major (the reduction runs over rows): the leading offset leads from one
-// 64-column block to the next.
-__device__ __forceinline__ uint64_t column_descriptor(uint32_t address) {
-  return kDescriptor | (uint64_t)(16384 >> 4) << 16 | address >> 4;
+// The upper word of a descriptor: 1024 bytes from 8 rows to the next 8, version,
+// 128-byte swizzle.
+constexpr uint32_t kDescriptorUp = 1024 >> 4 | 1u << 14 | 2u << 29;
+// The lower word. K-major (the reduction runs along a row): the leading offset is
+// not used. MN-major (it runs over rows): it leads from one 64-column block to
+// the next.
+__device__ __forceinline__ uint32_t row_descriptor(uint32_t address) { return 1u << 16 | address >> 4; }
+__device__ __forceinline__ uint32_t column_descriptor(uint32_t address) {
+  return (uint32_t)(16384 >> 4) << 16 | address >> 4;
 }
 
 // f16 operands, fp32 sums, M = 128; B is N x K along K, or along N.
@@ -185,20 +190,22 @@ template <int N, bool kBColumns>
 constexpr uint32_t kInstruction = 1u << 4 | (kBColumns ? 1u << 16 : 0u) | (uint32_t)(N / 8) << 17 |
                                   (uint32_t)(128 / 16) << 24;
 
-__device__ __forceinline__ void mma_shared(uint32_t d, uint64_t a, uint64_t b, uint32_t instruction,
+__device__ __forceinline__ void mma_shared(uint32_t d, uint32_t a, uint32_t b, uint32_t instruction,
                                            bool add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(instruction), "r"((uint32_t)add)
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(instruction), "r"((uint32_t)add), "r"(kDescriptorUp)
       : "memory");
 }
-__device__ __forceinline__ void mma_tensor(uint32_t d, uint32_t a, uint64_t b, uint32_t instruction,
+__device__ __forceinline__ void mma_tensor(uint32_t d, uint32_t a, uint32_t b, uint32_t instruction,
                                            bool add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(instruction), "r"((uint32_t)add)
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(instruction), "r"((uint32_t)add), "r"(kDescriptorUp)
       : "memory");
 }
 
@@ -277,10 +284,10 @@ template <int kRegisters>
 __device__ __forceinline__ void fewer_registers() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegisters));
 }
-// 512 threads are launched with 128 registers each; the shares of the four
-// warpgroups add up to 4 * 128.
-constexpr int kSoftmaxRegisters = 152, kConvertRegisters = 112, kIssueRegisters = 96;
-static_assert(2 * kSoftmaxRegisters + kConvertRegisters + kIssueRegisters == 4 * 128, "registers");
+// 640 threads are launched with 96 registers each; the shares of the five
+// warpgroups add up to 5 * 96.
+constexpr int kLaunchRegisters = 96, kSoftmaxRegisters = 136, kConvertRegisters = 72, kOtherRegisters = 64;
+static_assert(2 * kSoftmaxRegisters + 2 * kConvertRegisters + kOtherRegisters == 5 * kLaunchRegisters, "registers");
 
 // Chunk `chunk` (8 f16 values) of row `row` of an operand.
 template <int D>
@@ -314,22 +321,22 @@ __device__ __forceinline__ uint32_t pack_out(const Args& a, float x, float y) {
   return r;
 }
 
-// The next segment for a warp (or, in the issuing role, a thread), or null.
+// The next segment, or null.
 __device__ __forceinline__ const Work* take_work(Shared* sh, uint32_t n) {
   const Work* work = &sh->work[n % kWorkRing];
-  if (!bar_wait(&sh->work_full[n % kWorkRing], n / kWorkRing & 1, &sh->abort) || work->end < 0) return nullptr;
+  if (!bar_wait(&sh->work_full[n % kWorkRing], n / kWorkRing & 1) || work->end < 0) return nullptr;
   return work;
 }
 __device__ __forceinline__ void return_work(Shared* sh, uint32_t n) { bar_arrive(&sh->work_empty[n % kWorkRing]); }
 
-// --- warp 13 ---------------------------------------------------------------
+// --- warp 18 ---------------------------------------------------------------
 
 __device__ __forceinline__ void schedule_role(const Args& a, Walk<kThreads>& walk, Shared* sh) {
   uint32_t n = 0;
   Segment seg;
   for (bool more = true; more; ++n) {
     more = walk.next(a, &seg);
-    if (!bar_wait(&sh->work_empty[n % kWorkRing], (n / kWorkRing & 1) ^ 1, &sh->abort)) return;
+    if (!bar_wait(&sh->work_empty[n % kWorkRing], (n / kWorkRing & 1) ^ 1)) return;
     Work& w = sh->work[n % kWorkRing];
     w.end = -1;
     if (more) {
@@ -349,7 +356,7 @@ __device__ __forceinline__ void schedule_role(const Args& a, Walk<kThreads>& wal
   walk.finish(a);
 }
 
-// --- warps 8-11 ------------------------------------------------------------
+// --- warps 8-15 ------------------------------------------------------------
 
 // Volatile: it stays where it stands, a key tile ahead of its use.
 __device__ __forceinline__ uint4 load_global(const uint8_t* p) {
@@ -367,7 +374,6 @@ struct Convert {
   static constexpr int kRowsAPass = 128 / kChunks;
   const Args& a;
   Shared* sh;
-  uint32_t base;
   int t;  // thread of the warpgroup
 
   // Chunk and first row of this thread. Eight threads have four chunks of an
@@ -377,18 +383,28 @@ struct Convert {
   __device__ __forceinline__ int row0() const { return D == 128 ? t / 32 * 4 + t / 16 % 2 * 2 + t / 4 % 2 : t / 4; }
   __device__ __forceinline__ int row(int i) const { return row0() + kRowsAPass * i; }
 
-  // `place`: in lane g < 8, where 16-key group g begins in the cache (bytes, at
-  // this head), or negative when it has no page. `left`: keys of the tile that
-  // are read.
-  __device__ __forceinline__ void load(int kv, int64_t place, int left, uint4 (&raw)[kPasses]) const {
+  // Where this thread reads in a group that begins at byte 0 of the cache.
+  __device__ __forceinline__ int64_t from(int64_t row_bytes) const {
+    return row0() % 16 * row_bytes + chunk() * 16;
+  }
+  // The rows of a tile that stand below `left`, zeros for the others.
+  __device__ __forceinline__ void load(const uint8_t* cache, const Tile& tile, int left, uint4 (&raw)[kPasses]) const {
     const int64_t row_bytes = (int64_t)a.kv_heads * D;
-    const uint8_t* from =
-        (kv != 0 ? a.cache[1] : a.cache[0]) + row0() % 16 * row_bytes + chunk() * 16;
+    if (tile.run) {
+      const uint8_t* at = cache + tile.place[0] + row0() * row_bytes + chunk() * 16;
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      const int64_t at = __shfl_sync(0xFFFFFFFFu, place, row(i) / 16);
-      raw[i] = make_uint4(0, 0, 0, 0);
-      if (row(i) < left && at >= 0) raw[i] = load_global(from + at);
+      for (int i = 0; i < kPasses; ++i) {
+        raw[i] = load_global(at);
+        at += kRowsAPass * row_bytes;
+      }
+    } else {
+      const uint8_t* at = cache + row0() % 16 * row_bytes + chunk() * 16;
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        const int64_t group = tile.place[row(i) / 16];
+        raw[i] = make_uint4(0, 0, 0, 0);
+        if (row(i) < left && group >= 0) raw[i] = load_global(at + group);
+      }
     }
   }
 
@@ -425,153 +441,180 @@ struct Convert {
   }
 };
 
-template <int D>
+template <int D, bool kV>
 __device__ __forceinline__ void convert_role(const Args& a, Shared* sh, uint8_t* smem) {
-  Convert<D> c{a, sh, smem_of(smem), (int)threadIdx.x % 128};
-  constexpr int kPasses = Convert<D>::kPasses;
   using L = Layout<D>;
+  constexpr int kPasses = Convert<D>::kPasses;
+  Convert<D> c{a, sh, (int)threadIdx.x % 128};
+  const uint32_t operand = smem_of(smem) + (kV ? L::kV : L::kK);
+  const uint8_t* cache = kV ? a.cache[1] : a.cache[0];
+  uint64_t* full = kV ? sh->v_full : sh->k_full;
+  uint64_t* empty = kV ? sh->v_empty : sh->k_empty;
+  uint32_t count = 0;  // key tiles so far, over all segments
+  for (uint32_t n = 0;; ++n) {
+    const Work* work = take_work(sh, n);
+    if (__any_sync(0xFFFFFFFFu, work == nullptr)) return;
+    const int begin = work->begin, end = work->end, keys = work->keys;
+    uint4 raw[kPasses];
+    // Tile `tile` is put into shared memory, then tile + 1 is loaded: loads in
+    // flight would be waited for by the fence and the arrival.
+#pragma unroll 1
+    for (int tile = begin - 1; tile < end; ++tile) {
+      if (tile >= begin) {
+        const int stage = count % kStages;
+        if (!warp_wait(&empty[stage], (count / kStages & 1) ^ 1)) return;
+        if (kV && work->mixed(tile)) c.take_nan(stage, count, raw, smem + L::kNan + stage * L::kNanBytes);
+        c.put(operand + stage * L::kOperand, raw);
+        async_fence();
+        warp_arrive(&full[stage]);
+        ++count;
+      }
+      if (tile + 1 < end) {
+        if (!warp_wait(&sh->tile_full[count % kTileRing], count / kTileRing & 1)) return;
+        c.load(cache, sh->tiles[count % kTileRing], keys - (tile + 1) * kKeyTile, raw);
+      }
+    }
+    __syncwarp();
+    if (threadIdx.x % 32 == 0) return_work(sh, n);
+  }
+}
+
+// --- warp 19 ---------------------------------------------------------------
+
+// Lane g < 8 has 16-key group g of each tile. Entry n + 4 of the ring is written
+// when the scores of tile n + 2 are complete: they were issued after the output
+// of tile n + 1, so the softmax of tile n is done with its scales, and K and V of
+// tile n are loaded.
+template <int D>
+__device__ __forceinline__ void tile_role(const Args& a, Shared* sh) {
   const int lane = threadIdx.x % 32;
   const int blocks = a.page / 16 / a.block_tiles;  // scale blocks of a page
-  uint32_t count = 0;  // key tiles so far, over all segments
+  const bool long_pages = a.page % kKeyTile == 0;
+  uint32_t count = 0;
   for (uint32_t n = 0;; ++n) {
     const Work* work = take_work(sh, n);
     if (__any_sync(0xFFFFFFFFu, work == nullptr)) return;
     const int32_t* table = a.tables + work->seq * a.table_stride;
     const int begin = work->begin, end = work->end, keys = work->keys, head = work->head;
-    // Lane g < 8 of each warp has the page of group g of a tile (checked when it
-    // is used, a tile later), and from it where the group's rows and scales begin.
-    auto page_of = [&](int tile) {
+    auto page_of = [&](int tile) {  // checked when it is used, a tile later
       const int key = tile * kKeyTile + lane * 16;
-      return lane < 8 && tile < end && key < keys ? __ldg(table + key / a.page) : -1;
+      return lane < 8 && tile < end && key < keys ? __ldg(table + page_index(a, key)) : -1;
     };
     int page_next = page_of(begin);
-    int64_t place = -1;
-    float k_scale = 0.0f, v_scale = 0.0f, largest = -200.0f;
-    uint32_t absent = 0;
-    uint4 k_raw[kPasses], v_raw[kPasses];
-    // Tile `tile` is put into shared memory while tile + 1 is loaded.
+    float largest = -200.0f;
 #pragma unroll 1
-    for (int tile = begin - 1; tile < end; ++tile) {
-      if (tile >= begin) {
-        const int stage = count % kStages;
-        const uint32_t parity = (count / kStages & 1) ^ 1;
-        if (!warp_wait(&sh->k_empty[stage], parity, &sh->abort)) return;
-        c.put(c.base + L::kK + stage * L::kOperand, k_raw);
-        if (c.t < 32) {
-          Scales& s = sh->scales[count % kScaleRing];
-          const float log2 = v_scale > 0.0f ? log2f(v_scale) : v_scale == v_scale ? -200.0f : v_scale;
-          float most = lane < 8 ? log2 : -200.0f;
+    for (int tile = begin; tile < end; ++tile, ++count) {
+      const int page = page_next < a.num_pages ? page_next : -1;
+      page_next = page_of(tile + 1);
+      int64_t place = -1;
+      float k_scale = 0.0f, v_scale = 0.0f;
+      if (page >= 0) {
+        const int key = tile * kKeyTile + lane * 16, in_page = key - page_index(a, key) * a.page;
+        place = (((int64_t)page * a.page + in_page) * a.kv_heads + head) * D;
+        const int64_t at = ((int64_t)page * blocks + in_page / 16 / a.block_tiles) * a.kv_heads + head;
+        k_scale = __ldg(a.scale[0] + at);
+        v_scale = __ldg(a.scale[1] + at);
+      }
+      const uint32_t absent = __ballot_sync(0xFFFFFFFFu, page < 0) & 0xFFu;
+      const float log2 = v_scale > 0.0f ? log2f(v_scale) : v_scale == v_scale ? -200.0f : v_scale;
+      float most = lane < 8 ? log2 : -200.0f;
 #pragma unroll
-          for (int d = 4; d > 0; d /= 2) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
-          largest = fmaxf(largest, __shfl_sync(0xFFFFFFFFu, most, 0));
-          if (lane < 8) {
-            const float relative = log2 - largest;
-            const float shift = (relative < kLeastLog2 ? kLeastLog2 : relative) + kWeightLog2;
-            s.k[lane] = k_scale;
-            s.shift[lane] = shift;
-            s.inverse[lane] = exp2_fast(-shift);
-          }
-          if (lane == 0) {
-            s.largest = largest;
-            s.absent = absent;
-          }
-          __syncwarp();
-          if (lane == 0) bar_arrive(&sh->scale_full[count % kScaleRing]);
-        }
-        async_fence();
-        bar_arrive(&sh->k_full[stage]);
-        if (!warp_wait(&sh->v_empty[stage], parity, &sh->abort)) return;
-        if (work->mixed(tile)) c.take_nan(stage, count, v_raw, smem + L::kNan + stage * L::kNanBytes);
-        c.put(c.base + L::kV + stage * L::kOperand, v_raw);
-        async_fence();
-        bar_arrive(&sh->v_full[stage]);
-        ++count;
+      for (int d = 4; d > 0; d /= 2) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
+      largest = fmaxf(largest, __shfl_sync(0xFFFFFFFFu, most, 0));
+      if (count >= 2) {  // each phase in turn: a wait tells the last two apart only
+        const uint32_t scores = count - 2;
+        if (!warp_wait(&sh->k_empty[scores % kStages], scores / kStages & 1)) return;
       }
-      if (tile + 1 < end) {
-        const int page = page_next < a.num_pages ? page_next : -1;
-        page_next = page_of(tile + 2);
-        place = -1;
-        k_scale = v_scale = 0.0f;
-        if (page >= 0) {
-          const int in_page = ((tile + 1) * kKeyTile + lane * 16) % a.page;
-          place = ((int64_t)page * a.page + in_page) * a.kv_heads * D + head * D;
-          const int64_t at = ((int64_t)page * blocks + in_page / 16 / a.block_tiles) * a.kv_heads + head;
-          k_scale = __ldg(a.scale[0] + at);
-          v_scale = __ldg(a.scale[1] + at);
-        }
-        absent = __ballot_sync(0xFFFFFFFFu, page < 0) & 0xFFu;
-        c.load(0, place, keys - (tile + 1) * kKeyTile, k_raw);
-        c.load(1, place, keys - (tile + 1) * kKeyTile, v_raw);
+      Tile& t = sh->tiles[count % kTileRing];
+      if (lane < 8) {
+        const float relative = log2 - largest;
+        const float shift = (relative < kLeastLog2 ? kLeastLog2 : relative) + kWeightLog2;
+        t.place[lane] = place;
+        t.k[lane] = k_scale;
+        t.shift[lane] = shift;
+        t.inverse[lane] = exp2_fast(-shift);
       }
+      if (lane == 0) {
+        t.largest = largest;
+        t.absent = absent;
+        t.run = long_pages && keys - tile * kKeyTile >= kKeyTile && absent == 0;
+      }
+      __syncwarp();
+      if (lane == 0) bar_arrive(&sh->tile_full[count % kTileRing]);
     }
     __syncwarp();
     if (lane == 0) return_work(sh, n);
   }
 }
 
-// --- warp 12 ---------------------------------------------------------------
+// --- warps 16, 17 ----------------------------------------------------------
 
+// One thread for each 128-row tile g.
 template <int D>
-__device__ __forceinline__ void issue_role(Shared* sh, uint32_t base) {
+__device__ __forceinline__ void issue_role(Shared* sh, uint32_t base, int g) {
   using L = Layout<D>;
-  const uint32_t tmem = sh->tmem;
-  uint32_t count = 0;                // key tiles so far
-  uint32_t turn[2] = {0, 0}, segment[2] = {0, 0};
+  const uint32_t scores = sh->tmem + kScoresAt + g * kGroupColumns, output = sh->tmem + kOutputsAt + g * kGroupColumns;
+  const uint32_t q = row_descriptor(base + L::kQ + g * L::kOperand);
+  const uint32_t k0 = row_descriptor(base + L::kK), v0 = column_descriptor(base + L::kV);
+  uint32_t count = 0, turn = 0, segment = 0;  // key tiles so far, of the CTA and of this row tile
   for (uint32_t n = 0;; ++n) {
     const Work* work = take_work(sh, n);
     if (work == nullptr) return;
-    const int groups = work->groups(), tiles = work->end - work->begin;
+    const int tiles = work->end - work->begin;
+    const bool idle = g >= work->groups();
     return_work(sh, n);
-    // Step i: the output of key tile i - 1, then the scores of tile i.
+    if (idle) {  // K and V are not read, but given back in their order
+      for (int i = 0; i < tiles; ++i, ++count) {
+        const uint32_t stage = count % kStages, parity = count / kStages & 1;
+        if (!bar_wait(&sh->k_full[stage], parity)) return;
+        bar_arrive(&sh->k_empty[stage]);
+        if (!bar_wait(&sh->v_full[stage], parity)) return;
+        bar_arrive(&sh->v_empty[stage]);
+      }
+      continue;
+    }
+    if (!bar_wait(&sh->q_full[g], segment & 1)) return;
+    ++segment;
+    // Step h: the output of half h - 2, then the scores of half h in its columns.
 #pragma unroll 1
-    for (int i = 0; i <= tiles; ++i) {
-      const uint32_t now = count + i, before = now - 1;
-#pragma unroll 1
-      for (int g = 0; g < groups; ++g) {
-        const uint32_t scores = tmem + kScoresAt + g * kGroupColumns, output = tmem + kOutputsAt + g * kGroupColumns;
-        if (i > 0) {
-          if (!bar_wait(&sh->v_full[before % kStages], before / kStages & 1, &sh->abort)) return;
-          uint32_t& t = g == 0 ? turn[0] : turn[1];
-          if (!bar_wait(&sh->p_full[g], t & 1, &sh->abort)) return;
-          ++t;
-          tensor_fence_after();
-          const uint64_t v = column_descriptor(base + L::kV + before % kStages * L::kOperand);
+    for (int h = 0; h < 2 * tiles + 2; ++h) {
+      const uint32_t half = h & 1;
+      if (h >= 2) {
+        const uint32_t tile = count + (h - 2) / 2, stage = tile % kStages;
+        const uint32_t v = v0 + stage * (L::kOperand >> 4) + half * (kHalf * 128 >> 4);
+        if (half == 0 && !bar_wait(&sh->v_full[stage], tile / kStages & 1)) return;
+        if (!bar_wait(&sh->p_full[g][half], turn & 1)) return;
+        turn += half;
+        tensor_fence_after();
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            mma_tensor(output, scores + k * 8, v + (k * 2048 >> 4), kInstruction<D, true>, i > 1 || k > 0);
-          if (g == groups - 1) commit(&sh->v_empty[before % kStages]);
-          if (i == tiles) commit(&sh->o_full[g]);
-        }
-        if (i < tiles) {
-          if (!bar_wait(&sh->k_full[now % kStages], now / kStages & 1, &sh->abort)) return;
-          if (i == 0) {
-            uint32_t& t = g == 0 ? segment[0] : segment[1];
-            if (!bar_wait(&sh->q_full[g], t & 1, &sh->abort)) return;
-            ++t;
-          }
-          tensor_fence_after();
-          const uint64_t q = row_descriptor(base + L::kQ + g * L::kOperand);
-          const uint64_t keys = row_descriptor(base + L::kK + now % kStages * L::kOperand);
+        for (int k = 0; k < kHalf / 16; ++k)
+          mma_tensor(output, scores + half * kHalf + k * 8, v + (k * 2048 >> 4), kInstruction<D, true>, h > 2 || k > 0);
+        commit(&sh->o_done[g][half]);
+        if (half == 1) commit(&sh->v_empty[stage]);
+      }
+      if (h < 2 * tiles) {
+        const uint32_t tile = count + h / 2, stage = tile % kStages;
+        const uint32_t keys = k0 + stage * (L::kOperand >> 4) + half * (kHalf * 128 >> 4);
+        if (half == 0 && !bar_wait(&sh->k_full[stage], tile / kStages & 1)) return;
+        tensor_fence_after();
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t at = ((k / 4) * 16384 + (k % 4) * 32) >> 4;
-            mma_shared(scores, q + at, keys + at, kInstruction<128, false>, k > 0);
-          }
-          commit(&sh->s_full[g]);
-          if (g == groups - 1) commit(&sh->k_empty[now % kStages]);
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t at = ((k / 4) * 16384 + (k % 4) * 32) >> 4;
+          mma_shared(scores + half * kHalf, q + at, keys + at, kInstruction<kHalf, false>, k > 0);
         }
+        commit(&sh->s_full[g][half]);
+        if (half == 1) commit(&sh->k_empty[stage]);
       }
     }
     count += tiles;
   }
 }
 
-// --- warps 0-7 -------------------------------------------------------------
-
-// Scores behind the row's last key, or of groups without a page, become -inf.
+// Scores of a half behind the row's last key, or of groups without a page,
+// become -inf. `seen`, `absent`: of this half.
 __device__ __forceinline__ void mask_scores(uint32_t scores_at, int seen, uint32_t absent) {
 #pragma unroll 1
-  for (int c = 0; c < 4; ++c) {
+  for (int c = 0; c < kHalf / 32; ++c) {
     float s[32];
     load_begin(s, scores_at + 32 * c);
     load_end(s);
@@ -602,6 +645,49 @@ __device__ __forceinline__ float2 add_pair(float2 a, float2 b) {
 
 // --- warps 0-7 -------------------------------------------------------------
 
+// Log2 units of a raw score of group b. A scale of zero must not meet a masked
+// score's infinity.
+__device__ __forceinline__ float factor_of(const Tile& scales, int b, float factor) {
+  return fmaxf(scales.k[b] * factor, 1e-37f);
+}
+
+// The largest of the 32 scores of chunk c, in log2 units.
+__device__ __forceinline__ float top_of(const float (&s)[32], const Tile& scales, int c, float factor) {
+  float top[4] = {s[0], s[1], s[16], s[17]};
+#pragma unroll
+  for (int i = 2; i < 16; i += 2) {
+    top[0] = fmaxf(top[0], s[i]), top[1] = fmaxf(top[1], s[i + 1]);
+    top[2] = fmaxf(top[2], s[16 + i]), top[3] = fmaxf(top[3], s[17 + i]);
+  }
+  return fmaxf(fmaxf(top[0], top[1]) * factor_of(scales, 2 * c, factor),
+               fmaxf(top[2], top[3]) * factor_of(scales, 2 * c + 1, factor));
+}
+
+// P of the 32 scores of chunk c; its sums go into l. P takes the columns of
+// scores that have been read: 16 for these 32.
+__device__ __forceinline__ void weigh(const float (&s)[32], const Tile& scales, int c, float factor, float shift,
+                                      uint32_t scores_at, float& l) {
+  uint32_t p[16];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int b = 2 * c + k;
+    const float f = factor_of(scales, b, factor), bias = scales.shift[b] - shift;
+    float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0;
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const float2 x = exp2_pair(s[16 * k + i], s[16 * k + i + 1], f, bias);
+      const float2 y = exp2_pair(s[16 * k + i + 2], s[16 * k + i + 3], f, bias);
+      sum0 = add_pair(sum0, x);
+      sum1 = add_pair(sum1, y);
+      p[8 * k + i / 2] = pack_half(x.x, x.y);
+      p[8 * k + i / 2 + 1] = pack_half(y.x, y.y);
+    }
+    sum0 = add_pair(sum0, sum1);
+    l = fmaf(sum0.x + sum0.y, scales.inverse[b], l);
+  }
+  tensor_store16(scores_at + 16 * (c % 2), p);
+}
+
 template <int D>
 __device__ __forceinline__ void softmax_role(const Args& a, Shared* sh, uint8_t* smem) {
   using L = Layout<D>;
@@ -611,7 +697,7 @@ __device__ __forceinline__ void softmax_role(const Args& a, Shared* sh, uint8_t*
   const uint32_t scores_at = sh->tmem + lanes + kScoresAt + g * kGroupColumns;
   const uint32_t output_at = sh->tmem + lanes + kOutputsAt + g * kGroupColumns;
   const uint32_t q_at = base + L::kQ + g * L::kOperand;
-  uint32_t count = 0, turn = 0, segment = 0;
+  uint32_t count = 0, turn = 0;  // key tiles so far, of the CTA and of this row tile
   for (uint32_t n = 0;; ++n) {
     const Work* work = take_work(sh, n);
     if (__any_sync(0xFFFFFFFFu, work == nullptr)) return;
@@ -656,7 +742,7 @@ __device__ __forceinline__ void softmax_role(const Args& a, Shared* sh, uint8_t*
       }
       async_fence();
       tensor_fence_before();
-      bar_arrive(&sh->q_full[g]);
+      warp_arrive(&sh->q_full[g]);
     }
     float m = __uint_as_float(kNegInf), l = 0.0f, ref = -200.0f;  // ref: log2 of the largest V scale
     uint32_t nan[D / 32];
@@ -664,45 +750,32 @@ __device__ __forceinline__ void softmax_role(const Args& a, Shared* sh, uint8_t*
     for (int i = 0; i < D / 32; ++i) nan[i] = 0;
 
 #pragma unroll 1
-    for (int tile = begin; tile < end; ++tile, ++count) {
-      if (!warp_wait(&sh->scale_full[count % kScaleRing], count / kScaleRing & 1, &sh->abort)) return;
-      const Scales& scales = sh->scales[count % kScaleRing];
-      float f[8];
-#pragma unroll
-      for (int b = 0; b < 8; ++b)  // a scale of zero must not meet a masked score's infinity
-        f[b] = fmaxf(scales.k[b] * factor, 1e-37f);
-      const float largest = scales.largest;
-      const uint32_t absent = scales.absent;
-      const int seen = limit - tile * kKeyTile;  // of this tile's keys
-      const bool masked = __any_sync(0xFFFFFFFFu, seen < kKeyTile) || absent != 0;
-      if (!warp_wait(&sh->s_full[g], turn & 1, &sh->abort)) return;
-      ++turn;
+    for (int h = 2 * begin; h < 2 * end; ++h) {
+      const int tile = h / 2, half = h & 1;
+      // The scores first: a row tile that sat out segments may be ahead of the
+      // ring of tiles by more than its barriers can tell.
+      if (!warp_wait(&sh->s_full[g][half], turn & 1)) return;
       tensor_fence_after();
-      if (masked) mask_scores(scores_at, seen, absent);
-
-      // The row's maximum; then its scores again, which costs less than the
-      // registers to keep them.
-      float buffer[2][32];
-      float most = __uint_as_float(kNegInf);
-      load_begin(buffer[0], scores_at);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float(&s)[32] = buffer[c % 2];
-        load_end(s);
-        load_begin(buffer[(c + 1) % 2], scores_at + (c + 1) % 4 * 32);
-        float top[4] = {s[0], s[1], s[16], s[17]};
-#pragma unroll
-        for (int i = 2; i < 16; i += 2) {
-          top[0] = fmaxf(top[0], s[i]), top[1] = fmaxf(top[1], s[i + 1]);
-          top[2] = fmaxf(top[2], s[16 + i]), top[3] = fmaxf(top[3], s[17 + i]);
-        }
-        most = fmaxf(most, fmaxf(fmaxf(top[0], top[1]) * f[2 * c], fmaxf(top[2], top[3]) * f[2 * c + 1]));
-      }
-      load_end(buffer[0]);
+      if (half == 0 && !warp_wait(&sh->tile_full[count % kTileRing], count / kTileRing & 1)) return;
+      const Tile& scales = sh->tiles[count % kTileRing];
+      const float largest = scales.largest;
+      const uint32_t absent = scales.absent >> 4 * half & 0xFu;
+      const int seen = limit - h * kHalf;  // of this half's keys
+      const bool masked = __any_sync(0xFFFFFFFFu, seen < kHalf) || absent != 0;
+      const uint32_t half_at = scores_at + half * kHalf;
+      if (masked) mask_scores(half_at, seen, absent);
+      float x[32], y[32];
+      load_begin(x, half_at);
+      load_begin(y, half_at + 32);
+      load_end(x);
+      load_end(y);
+      const float most = fmaxf(top_of(x, scales, 2 * half, factor), top_of(y, scales, 2 * half + 1, factor));
       if (__any_sync(0xFFFFFFFFu, most > m + kRaise || largest > ref)) {
         const float top = fmaxf(m, most);
         const float keep_l = top == m ? 1.0f : exp2_fast(m - top);
-        if (tile != begin) {
+        if (h != 2 * begin) {  // not before the output of the half before is complete
+          if (!warp_wait(&sh->o_done[g][half ^ 1], (turn - (half ^ 1)) & 1)) return;
+          tensor_fence_after();
           const float keep = keep_l * exp2_fast(ref - largest);
 #pragma unroll 1
           for (int c = 0; c < D / 8; ++c) tensor_scale8(output_at + 8 * c, keep);
@@ -712,38 +785,15 @@ __device__ __forceinline__ void softmax_role(const Args& a, Shared* sh, uint8_t*
         ref = largest;
       }
       const float shift = m == __uint_as_float(kNegInf) ? 0.0f : m;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float(&s)[32] = buffer[c % 2];
-        if (c > 0) load_end(s);
-        if (c < 3) load_begin(buffer[(c + 1) % 2], scores_at + (c + 1) * 32);
-        uint32_t p[16];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int b = 2 * c + k;
-          const float bias = scales.shift[b] - shift;
-          float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0;
-#pragma unroll
-          for (int i = 0; i < 16; i += 4) {
-            const float2 x = exp2_pair(s[16 * k + i], s[16 * k + i + 1], f[b], bias);
-            const float2 y = exp2_pair(s[16 * k + i + 2], s[16 * k + i + 3], f[b], bias);
-            sum0 = add_pair(sum0, x);
-            sum1 = add_pair(sum1, y);
-            p[8 * k + i / 2] = pack_half(x.x, x.y);
-            p[8 * k + i / 2 + 1] = pack_half(y.x, y.y);
-          }
-          sum0 = add_pair(sum0, sum1);
-          l = fmaf(sum0.x + sum0.y, scales.inverse[b], l);
-        }
-        // P takes the columns of scores that have been read: 16 for these 32.
-        tensor_store16(scores_at + 16 * c, p);
-      }
+      weigh(x, scales, 2 * half, factor, shift, half_at, l);
+      weigh(y, scales, 2 * half + 1, factor, shift, half_at, l);
       if (work->mixed(tile)) {
         const int stage = count % kStages;
-        if (!warp_wait(&sh->v_full[stage], count / kStages & 1, &sh->abort)) return;
+        if (!warp_wait(&sh->v_full[stage], count / kStages & 1)) return;
         if (*reinterpret_cast<volatile uint32_t*>(&sh->nan[stage]) == count + 1) {
-          const uint32_t* masks = reinterpret_cast<const uint32_t*>(smem + L::kNan + stage * L::kNanBytes);
-          for (int i = 0; i < min(seen, kKeyTile); ++i)
+          const uint32_t* masks = reinterpret_cast<const uint32_t*>(smem + L::kNan + stage * L::kNanBytes) +
+                                  half * kHalf * (D / 32);
+          for (int i = 0; i < min(seen, kHalf); ++i)
 #pragma unroll
             for (int w = 0; w < D / 32; ++w) nan[w] |= masks[i * (D / 32) + w];
           __syncwarp();
@@ -751,11 +801,12 @@ __device__ __forceinline__ void softmax_role(const Args& a, Shared* sh, uint8_t*
       }
       tensor_wait_stores();
       tensor_fence_before();
-      bar_arrive(&sh->p_full[g]);
+      warp_arrive(&sh->p_full[g][half]);
+      turn += half;
+      count += half;
     }
 
-    if (!warp_wait(&sh->o_full[g], segment & 1, &sh->abort)) return;
-    ++segment;
+    if (!warp_wait(&sh->o_done[g][1], (turn - 1) & 1)) return;
     tensor_fence_after();
     // exp2(ref) may be as small as a scale can be; a row of zero scales is zero.
     const bool whole = work->slot < 0;
@@ -820,28 +871,29 @@ __global__ void __launch_bounds__(kThreads, 1) attention_extend_fp8_kernel(const
   const int warp = threadIdx.x / 32;
   if (threadIdx.x == 0) {
     for (int g = 0; g < 2; ++g) {
-      bar_init(&sh.q_full[g], 128);
-      bar_init(&sh.s_full[g], 1);
-      bar_init(&sh.p_full[g], 128);
-      bar_init(&sh.o_full[g], 1);
+      bar_init(&sh.q_full[g], 4);  // one for each warp
+      for (int h = 0; h < 2; ++h) {
+        bar_init(&sh.s_full[g][h], 1);
+        bar_init(&sh.p_full[g][h], 4);
+        bar_init(&sh.o_done[g][h], 1);
+      }
     }
     for (int i = 0; i < kStages; ++i) {
-      bar_init(&sh.k_full[i], 128);
-      bar_init(&sh.k_empty[i], 1);
-      bar_init(&sh.v_full[i], 128);
-      bar_init(&sh.v_empty[i], 1);
+      bar_init(&sh.k_full[i], 4);
+      bar_init(&sh.k_empty[i], 2);  // one for each row tile
+      bar_init(&sh.v_full[i], 4);
+      bar_init(&sh.v_empty[i], 2);
     }
-    for (int i = 0; i < kScaleRing; ++i) bar_init(&sh.scale_full[i], 1);
+    for (int i = 0; i < kTileRing; ++i) bar_init(&sh.tile_full[i], 1);
     for (int i = 0; i < kWorkRing; ++i) {
       bar_init(&sh.work_full[i], 1);
-      bar_init(&sh.work_empty[i], 13);  // warps 0-11 and the issuing thread
+      bar_init(&sh.work_empty[i], 19);  // all warps but the scheduler
     }
-    bar_init(&sh.drained, 1);
-    sh.abort = 0;
+    for (int g = 0; g < 2; ++g) bar_init(&sh.drained[g], 1);
     sh.nan[0] = sh.nan[1] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 12) {
+  if (warp == 16) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_of(&sh.tmem)),
                  "r"(kTmemColumns)
                  : "memory");
@@ -857,25 +909,30 @@ __global__ void __launch_bounds__(kThreads, 1) attention_extend_fp8_kernel(const
     softmax_role<D>(a, &sh, smem);
   } else if (warp < 12) {
     fewer_registers<kConvertRegisters>();
-    convert_role<D>(a, &sh, smem);
+    convert_role<D, false>(a, &sh, smem);
+  } else if (warp < 16) {
+    fewer_registers<kConvertRegisters>();
+    convert_role<D, true>(a, &sh, smem);
   } else {
-    fewer_registers<kIssueRegisters>();
-    if (threadIdx.x == 12 * 32) {
-      issue_role<D>(&sh, smem_of(smem));
-      // Nothing of this CTA's is in flight when its tensor memory is freed.
-      commit(&sh.drained);
-      bool done = bar_try(&sh.drained, 0);
-      for (int spins = 0; !done && spins < 1 << 20; ++spins) done = bar_try(&sh.drained, 0);
-      if (!done) atomicOr(&g_extend_error, kErrExtendWaitTimeout);
-    } else if (threadIdx.x == 13 * 32) {
-      schedule_role(a, walk, &sh);
+    fewer_registers<kOtherRegisters>();
+    if (warp < 18) {
+      if (threadIdx.x % 32 == 0) {
+        issue_role<D>(&sh, smem_of(smem), warp - 16);
+        // Nothing of this CTA's is in flight when its tensor memory is freed.
+        commit(&sh.drained[warp - 16]);
+        bar_wait(&sh.drained[warp - 16], 0);
+      }
+    } else if (warp == 18) {
+      if (threadIdx.x % 32 == 0) schedule_role(a, walk, &sh);
+    } else {
+      tile_role<D>(a, &sh);
     }
     __syncwarp();
   }
   tensor_fence_before();
   __syncthreads();
   tensor_fence_after();
-  if (warp == 12)
+  if (warp == 16)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(sh.tmem), "r"(kTmemColumns));
 }
 

@@ -203,6 +203,9 @@ extern "C" int kvoff_attention_fp8(
   a.num_pages = (int32_t)num_pages;
   a.page = (int32_t)page_size;
   a.block_tiles = (int32_t)(scale_block / 16);
+  a.page_shift = -1;
+  if ((page_size & (page_size - 1)) == 0)
+    for (a.page_shift = 0; (1ll << a.page_shift) < page_size;) ++a.page_shift;
   a.seqs = (int32_t)num_seqs;
   a.num_tokens = (int32_t)num_tokens;
   a.q_heads = (int32_t)q_heads;

@@ -28,6 +28,7 @@ struct Args {
   const int32_t* starts;  // null: token s is sequence s
   float scale_log2;       // softmax scale * log2(e)
   int32_t table_width, num_pages, page, block_tiles;  // scale block in 16-key units
+  int32_t page_shift;  // log2 of page, or -1 when it is no power of two
   int32_t seqs, num_tokens, q_heads, kv_heads, group;
   int32_t rows;      // packed rows of a row tile
   int32_t fixed;     // what beginning and ending a row tile costs, as keys read
@@ -38,6 +39,11 @@ struct Args {
   float* partial;            // 2 slots per CTA
   struct Record* records;    // one per CTA
 };
+
+// Page of a key, and the key's place in it. A division takes 30 instructions.
+__device__ __forceinline__ int page_index(const Args& a, int key) {
+  return a.page_shift >= 0 ? key >> a.page_shift : key / a.page;
+}
 
 // What a CTA leaves for the join: the split (sequence, head, row tile) that
 // begins in it, how many CTAs after it hold parts of it, and which of its two

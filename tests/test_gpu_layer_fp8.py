@@ -8,6 +8,7 @@ import math
 import pytest
 import torch
 
+import kvoff
 import layer_reference as ref
 from kvoff import attention as layer
 from kvoff import ops
@@ -16,6 +17,13 @@ pytestmark = pytest.mark.gpu
 
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
 NAN_BYTE = 0x7F
+
+
+@pytest.fixture(autouse=True)
+def _no_wait_ran_out(cuda):
+    """Each bounded wait inside a kernel ended because what it waited for came."""
+    yield
+    assert kvoff.device_error(0) == 0
 
 
 def generator(seed):
