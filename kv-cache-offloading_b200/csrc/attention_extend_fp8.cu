@@ -32,7 +32,7 @@
 // wait for products. Rescaling O waits for the output of the half before.
 //
 // Every wait is bounded; one that runs out sets an error flag that
-// kvoff_device_error reads, and all roles leave.
+// kvoff_device_error reads; the kernel then ends without waiting for anything.
 #include "attention_fp8.h"
 #include "codec.cuh"
 
@@ -131,9 +131,14 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
   __syncwarp();
   if (threadIdx.x % 32 == 0) bar_arrive(bar);
 }
-// Waits for the phase of `parity`, at most kMostWaits times kWaitNs. False: the
-// error flag is set and the role leaves, after which the others run out too.
-__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity) {
+// Waits for the phase of `parity`, at most kMostWaits times kWaitNs. When that
+// runs out the error flag is set and the thread goes on: what it computes then
+// means nothing, but each later wait of its ends at its first look (`most` is 0),
+// so the kernel ends, and no warp is torn apart on the way.
+struct Patience {
+  uint32_t most = kMostWaits;
+};
+__device__ __forceinline__ void bar_wait(uint64_t* bar, uint32_t parity, Patience& patience) {
   uint32_t done;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\tmov.u32 n, 0;\n"
@@ -146,14 +151,12 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity) {
       "DONE:\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(done)
-      : "r"(smem_of(bar)), "r"(parity), "r"(kWaitNs), "n"(kMostWaits)
+      : "r"(smem_of(bar)), "r"(parity), "r"(kWaitNs), "r"(patience.most)
       : "memory");
-  if (done == 0) atomicOr(&g_extend_error, kErrExtendWaitTimeout);
-  return done != 0;
-}
-// The same for a whole warp, whose lanes stay or leave together.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
-  return __all_sync(0xFFFFFFFFu, bar_wait(bar, parity));
+  if (done == 0) {
+    if (patience.most != 0) atomicOr(&g_extend_error, kErrExtendWaitTimeout);
+    patience.most = 0;
+  }
 }
 
 __device__ __forceinline__ void tensor_fence_before() {
@@ -321,22 +324,24 @@ __device__ __forceinline__ uint32_t pack_out(const Args& a, float x, float y) {
   return r;
 }
 
-// The next segment, or null.
-__device__ __forceinline__ const Work* take_work(Shared* sh, uint32_t n) {
+// The next segment, or null (also when a wait has run out).
+__device__ __forceinline__ const Work* take_work(Shared* sh, uint32_t n, Patience& patience) {
   const Work* work = &sh->work[n % kWorkRing];
-  if (!bar_wait(&sh->work_full[n % kWorkRing], n / kWorkRing & 1) || work->end < 0) return nullptr;
-  return work;
+  bar_wait(&sh->work_full[n % kWorkRing], n / kWorkRing & 1, patience);
+  return patience.most == 0 || work->end < 0 ? nullptr : work;
 }
 __device__ __forceinline__ void return_work(Shared* sh, uint32_t n) { bar_arrive(&sh->work_empty[n % kWorkRing]); }
 
 // --- warp 18 ---------------------------------------------------------------
 
 __device__ __forceinline__ void schedule_role(const Args& a, Walk<kThreads>& walk, Shared* sh) {
+  Patience patience;
   uint32_t n = 0;
   Segment seg;
   for (bool more = true; more; ++n) {
     more = walk.next(a, &seg);
-    if (!bar_wait(&sh->work_empty[n % kWorkRing], (n / kWorkRing & 1) ^ 1)) return;
+    bar_wait(&sh->work_empty[n % kWorkRing], (n / kWorkRing & 1) ^ 1, patience);
+    if (patience.most == 0) return;
     Work& w = sh->work[n % kWorkRing];
     w.end = -1;
     if (more) {
@@ -441,18 +446,21 @@ struct Convert {
   }
 };
 
-template <int D, bool kV>
-__device__ __forceinline__ void convert_role(const Args& a, Shared* sh, uint8_t* smem) {
+// K and V run the same code: what the roles execute in each tile has to stay in the
+// instruction cache together.
+template <int D>
+__device__ __forceinline__ void convert_role(const Args& a, Shared* sh, uint8_t* smem, bool is_v) {
   using L = Layout<D>;
   constexpr int kPasses = Convert<D>::kPasses;
   Convert<D> c{a, sh, (int)threadIdx.x % 128};
-  const uint32_t operand = smem_of(smem) + (kV ? L::kV : L::kK);
-  const uint8_t* cache = kV ? a.cache[1] : a.cache[0];
-  uint64_t* full = kV ? sh->v_full : sh->k_full;
-  uint64_t* empty = kV ? sh->v_empty : sh->k_empty;
+  const uint32_t operand = smem_of(smem) + (is_v ? L::kV : L::kK);
+  const uint8_t* cache = is_v ? a.cache[1] : a.cache[0];
+  uint64_t* full = is_v ? sh->v_full : sh->k_full;
+  uint64_t* empty = is_v ? sh->v_empty : sh->k_empty;
+  Patience patience;
   uint32_t count = 0;  // key tiles so far, over all segments
   for (uint32_t n = 0;; ++n) {
-    const Work* work = take_work(sh, n);
+    const Work* work = take_work(sh, n, patience);
     if (__any_sync(0xFFFFFFFFu, work == nullptr)) return;
     const int begin = work->begin, end = work->end, keys = work->keys;
     uint4 raw[kPasses];
@@ -462,16 +470,17 @@ __device__ __forceinline__ void convert_role(const Args& a, Shared* sh, uint8_t*
     for (int tile = begin - 1; tile < end; ++tile) {
       if (tile >= begin) {
         const int stage = count % kStages;
-        if (!warp_wait(&empty[stage], (count / kStages & 1) ^ 1)) return;
-        if (kV && work->mixed(tile)) c.take_nan(stage, count, raw, smem + L::kNan + stage * L::kNanBytes);
+        bar_wait(&empty[stage], (count / kStages & 1) ^ 1, patience);
+        if (is_v && work->mixed(tile)) c.take_nan(stage, count, raw, smem + L::kNan + stage * L::kNanBytes);
         c.put(operand + stage * L::kOperand, raw);
         async_fence();
         warp_arrive(&full[stage]);
         ++count;
       }
       if (tile + 1 < end) {
-        if (!warp_wait(&sh->tile_full[count % kTileRing], count / kTileRing & 1)) return;
-        c.load(cache, sh->tiles[count % kTileRing], keys - (tile + 1) * kKeyTile, raw);
+        bar_wait(&sh->tile_full[count % kTileRing], count / kTileRing & 1, patience);
+        if (patience.most != 0)  // else the entry may be anything
+          c.load(cache, sh->tiles[count % kTileRing], keys - (tile + 1) * kKeyTile, raw);
       }
     }
     __syncwarp();
@@ -490,9 +499,10 @@ __device__ __forceinline__ void tile_role(const Args& a, Shared* sh) {
   const int lane = threadIdx.x % 32;
   const int blocks = a.page / 16 / a.block_tiles;  // scale blocks of a page
   const bool long_pages = a.page % kKeyTile == 0;
+  Patience patience;
   uint32_t count = 0;
   for (uint32_t n = 0;; ++n) {
-    const Work* work = take_work(sh, n);
+    const Work* work = take_work(sh, n, patience);
     if (__any_sync(0xFFFFFFFFu, work == nullptr)) return;
     const int32_t* table = a.tables + work->seq * a.table_stride;
     const int begin = work->begin, end = work->end, keys = work->keys, head = work->head;
@@ -516,14 +526,16 @@ __device__ __forceinline__ void tile_role(const Args& a, Shared* sh) {
         v_scale = __ldg(a.scale[1] + at);
       }
       const uint32_t absent = __ballot_sync(0xFFFFFFFFu, page < 0) & 0xFFu;
-      const float log2 = v_scale > 0.0f ? log2f(v_scale) : v_scale == v_scale ? -200.0f : v_scale;
+      float log2;
+      asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(log2) : "f"(v_scale));
+      log2 = v_scale > 0.0f ? fmaxf(log2, -200.0f) : v_scale == v_scale ? -200.0f : v_scale;
       float most = lane < 8 ? log2 : -200.0f;
 #pragma unroll
       for (int d = 4; d > 0; d /= 2) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
       largest = fmaxf(largest, __shfl_sync(0xFFFFFFFFu, most, 0));
       if (count >= 2) {  // each phase in turn: a wait tells the last two apart only
         const uint32_t scores = count - 2;
-        if (!warp_wait(&sh->k_empty[scores % kStages], scores / kStages & 1)) return;
+        bar_wait(&sh->k_empty[scores % kStages], scores / kStages & 1, patience);
       }
       Tile& t = sh->tiles[count % kTileRing];
       if (lane < 8) {
@@ -556,9 +568,10 @@ __device__ __forceinline__ void issue_role(Shared* sh, uint32_t base, int g) {
   const uint32_t scores = sh->tmem + kScoresAt + g * kGroupColumns, output = sh->tmem + kOutputsAt + g * kGroupColumns;
   const uint32_t q = row_descriptor(base + L::kQ + g * L::kOperand);
   const uint32_t k0 = row_descriptor(base + L::kK), v0 = column_descriptor(base + L::kV);
+  Patience patience;
   uint32_t count = 0, turn = 0, segment = 0;  // key tiles so far, of the CTA and of this row tile
   for (uint32_t n = 0;; ++n) {
-    const Work* work = take_work(sh, n);
+    const Work* work = take_work(sh, n, patience);
     if (work == nullptr) return;
     const int tiles = work->end - work->begin;
     const bool idle = g >= work->groups();
@@ -566,14 +579,14 @@ __device__ __forceinline__ void issue_role(Shared* sh, uint32_t base, int g) {
     if (idle) {  // K and V are not read, but given back in their order
       for (int i = 0; i < tiles; ++i, ++count) {
         const uint32_t stage = count % kStages, parity = count / kStages & 1;
-        if (!bar_wait(&sh->k_full[stage], parity)) return;
+        bar_wait(&sh->k_full[stage], parity, patience);
         bar_arrive(&sh->k_empty[stage]);
-        if (!bar_wait(&sh->v_full[stage], parity)) return;
+        bar_wait(&sh->v_full[stage], parity, patience);
         bar_arrive(&sh->v_empty[stage]);
       }
       continue;
     }
-    if (!bar_wait(&sh->q_full[g], segment & 1)) return;
+    bar_wait(&sh->q_full[g], segment & 1, patience);
     ++segment;
     // Step h: the output of half h - 2, then the scores of half h in its columns.
 #pragma unroll 1
@@ -582,8 +595,8 @@ __device__ __forceinline__ void issue_role(Shared* sh, uint32_t base, int g) {
       if (h >= 2) {
         const uint32_t tile = count + (h - 2) / 2, stage = tile % kStages;
         const uint32_t v = v0 + stage * (L::kOperand >> 4) + half * (kHalf * 128 >> 4);
-        if (half == 0 && !bar_wait(&sh->v_full[stage], tile / kStages & 1)) return;
-        if (!bar_wait(&sh->p_full[g][half], turn & 1)) return;
+        if (half == 0) bar_wait(&sh->v_full[stage], tile / kStages & 1, patience);
+        bar_wait(&sh->p_full[g][half], turn & 1, patience);
         turn += half;
         tensor_fence_after();
 #pragma unroll
@@ -595,7 +608,7 @@ __device__ __forceinline__ void issue_role(Shared* sh, uint32_t base, int g) {
       if (h < 2 * tiles) {
         const uint32_t tile = count + h / 2, stage = tile % kStages;
         const uint32_t keys = k0 + stage * (L::kOperand >> 4) + half * (kHalf * 128 >> 4);
-        if (half == 0 && !bar_wait(&sh->k_full[stage], tile / kStages & 1)) return;
+        if (half == 0) bar_wait(&sh->k_full[stage], tile / kStages & 1, patience);
         tensor_fence_after();
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
@@ -697,9 +710,10 @@ __device__ __forceinline__ void softmax_role(const Args& a, Shared* sh, uint8_t*
   const uint32_t scores_at = sh->tmem + lanes + kScoresAt + g * kGroupColumns;
   const uint32_t output_at = sh->tmem + lanes + kOutputsAt + g * kGroupColumns;
   const uint32_t q_at = base + L::kQ + g * L::kOperand;
+  Patience patience;
   uint32_t count = 0, turn = 0;  // key tiles so far, of the CTA and of this row tile
   for (uint32_t n = 0;; ++n) {
-    const Work* work = take_work(sh, n);
+    const Work* work = take_work(sh, n, patience);
     if (__any_sync(0xFFFFFFFFu, work == nullptr)) return;
     const int begin = work->begin, end = work->end;
     if (g >= work->groups()) {
@@ -751,19 +765,18 @@ __device__ __forceinline__ void softmax_role(const Args& a, Shared* sh, uint8_t*
 
 #pragma unroll 1
     for (int h = 2 * begin; h < 2 * end; ++h) {
-      const int tile = h / 2, half = h & 1;
+      const int half = h & 1;
+      const uint32_t half_at = scores_at + half * kHalf;
       // The scores first: a row tile that sat out segments may be ahead of the
       // ring of tiles by more than its barriers can tell.
-      if (!warp_wait(&sh->s_full[g][half], turn & 1)) return;
+      bar_wait(&sh->s_full[g][half], turn & 1, patience);
       tensor_fence_after();
-      if (half == 0 && !warp_wait(&sh->tile_full[count % kTileRing], count / kTileRing & 1)) return;
+      if (half == 0) bar_wait(&sh->tile_full[count % kTileRing], count / kTileRing & 1, patience);
       const Tile& scales = sh->tiles[count % kTileRing];
       const float largest = scales.largest;
       const uint32_t absent = scales.absent >> 4 * half & 0xFu;
       const int seen = limit - h * kHalf;  // of this half's keys
-      const bool masked = __any_sync(0xFFFFFFFFu, seen < kHalf) || absent != 0;
-      const uint32_t half_at = scores_at + half * kHalf;
-      if (masked) mask_scores(half_at, seen, absent);
+      if (__any_sync(0xFFFFFFFFu, seen < kHalf) || absent != 0) mask_scores(half_at, seen, absent);
       float x[32], y[32];
       load_begin(x, half_at);
       load_begin(y, half_at + 32);
@@ -774,7 +787,7 @@ __device__ __forceinline__ void softmax_role(const Args& a, Shared* sh, uint8_t*
         const float top = fmaxf(m, most);
         const float keep_l = top == m ? 1.0f : exp2_fast(m - top);
         if (h != 2 * begin) {  // not before the output of the half before is complete
-          if (!warp_wait(&sh->o_done[g][half ^ 1], (turn - (half ^ 1)) & 1)) return;
+          bar_wait(&sh->o_done[g][half ^ 1], (turn - (half ^ 1)) & 1, patience);
           tensor_fence_after();
           const float keep = keep_l * exp2_fast(ref - largest);
 #pragma unroll 1
@@ -787,9 +800,9 @@ __device__ __forceinline__ void softmax_role(const Args& a, Shared* sh, uint8_t*
       const float shift = m == __uint_as_float(kNegInf) ? 0.0f : m;
       weigh(x, scales, 2 * half, factor, shift, half_at, l);
       weigh(y, scales, 2 * half + 1, factor, shift, half_at, l);
-      if (work->mixed(tile)) {
+      if (work->mixed(h / 2)) {
         const int stage = count % kStages;
-        if (!warp_wait(&sh->v_full[stage], count / kStages & 1)) return;
+        bar_wait(&sh->v_full[stage], count / kStages & 1, patience);
         if (*reinterpret_cast<volatile uint32_t*>(&sh->nan[stage]) == count + 1) {
           const uint32_t* masks = reinterpret_cast<const uint32_t*>(smem + L::kNan + stage * L::kNanBytes) +
                                   half * kHalf * (D / 32);
@@ -806,7 +819,7 @@ __device__ __forceinline__ void softmax_role(const Args& a, Shared* sh, uint8_t*
       count += half;
     }
 
-    if (!warp_wait(&sh->o_done[g][1], (turn - 1) & 1)) return;
+    bar_wait(&sh->o_done[g][1], (turn - 1) & 1, patience);
     tensor_fence_after();
     // exp2(ref) may be as small as a scale can be; a row of zero scales is zero.
     const bool whole = work->slot < 0;
@@ -907,12 +920,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_extend_fp8_kernel(const
   if (warp < 8) {
     more_registers<kSoftmaxRegisters>();
     softmax_role<D>(a, &sh, smem);
-  } else if (warp < 12) {
-    fewer_registers<kConvertRegisters>();
-    convert_role<D, false>(a, &sh, smem);
   } else if (warp < 16) {
     fewer_registers<kConvertRegisters>();
-    convert_role<D, true>(a, &sh, smem);
+    convert_role<D>(a, &sh, smem, warp >= 12);
   } else {
     fewer_registers<kOtherRegisters>();
     if (warp < 18) {
@@ -920,7 +930,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_extend_fp8_kernel(const
         issue_role<D>(&sh, smem_of(smem), warp - 16);
         // Nothing of this CTA's is in flight when its tensor memory is freed.
         commit(&sh.drained[warp - 16]);
-        bar_wait(&sh.drained[warp - 16], 0);
+        Patience patience;
+        bar_wait(&sh.drained[warp - 16], 0, patience);
       }
     } else if (warp == 18) {
       if (threadIdx.x % 32 == 0) schedule_role(a, walk, &sh);
