@@ -407,6 +407,17 @@ KVOFF_API int kvoff_attention_fp8_workspace(int64_t num_seqs, int64_t max_seqlen
                                             int64_t* bytes);
 
 /*
+ * The three calls of a layer above with their parameters in one array, in the
+ * order of the declarations: integers, pointers and the stream as int64, the
+ * softmax scale as the bits of a double. For hosts that pay for each argument of
+ * a foreign call (twenty of them cost a ctypes caller 6 us, more than the
+ * kernels of a decode step). Counts: 21, 17 and 28.
+ */
+KVOFF_API int kvoff_rotary_packed(const int64_t* args);
+KVOFF_API int kvoff_store_kvcache_fp8_packed(const int64_t* args);
+KVOFF_API int kvoff_attention_fp8_packed(const int64_t* args);
+
+/*
  * Pinned host slab: mmap `bytes`, prefer NUMA node `numa_node` (-1: no
  * preference), page-lock it with cudaHostRegister(Portable | Mapped) and
  * return the host pointer and its device alias for zero-copy kernels.

@@ -553,15 +553,12 @@ __global__ void __launch_bounds__(kThreads, 2) attention_decode_fp8_kernel(const
 
 template <int D, int NT>
 int launch(const Args& a, int grid, cudaStream_t stream) {
-  const auto kernel = attention_decode_fp8_kernel<D, NT>;
   constexpr int kRing = kWarps * Shape<D>::kWarpBytes;
   constexpr int kSums = kWarps * 8 * NT * (D + 4) * (int)sizeof(float);
   constexpr int kBytes = kRing > kSums ? kRing : kSums;
   static_assert(kBytes <= 112 * 1024, "two CTAs an SM");
-  KVOFF_TRY(cuda_status(
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes),
-      "attention_fp8 shared memory"));
-  kernel<<<grid, kThreads, kBytes, stream>>>(a);
+  KVOFF_TRY((allow_shared<attention_decode_fp8_kernel<D, NT>>(kBytes)));
+  attention_decode_fp8_kernel<D, NT><<<grid, kThreads, kBytes, stream>>>(a);
   return cuda_status(cudaGetLastError(), "attention_fp8 launch");
 }
 

@@ -949,11 +949,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_extend_fp8_kernel(const
 
 template <int D>
 int launch(const Args& a, int grid, cudaStream_t stream) {
-  const auto kernel = attention_extend_fp8_kernel<D>;
-  KVOFF_TRY(cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             Layout<D>::kBytes),
-                        "attention_fp8 shared memory"));
-  kernel<<<grid, kThreads, Layout<D>::kBytes, stream>>>(a);
+  KVOFF_TRY(allow_shared<attention_extend_fp8_kernel<D>>(Layout<D>::kBytes));
+  attention_extend_fp8_kernel<D><<<grid, kThreads, Layout<D>::kBytes, stream>>>(a);
   return cuda_status(cudaGetLastError(), "attention_fp8 launch");
 }
 

@@ -2,6 +2,8 @@
 // whose keys were read by several CTAs.
 #include "attention_fp8.h"
 
+#include <string.h>
+
 namespace kvoff {
 namespace attention {
 namespace {
@@ -225,4 +227,19 @@ extern "C" int kvoff_attention_fp8(
                      : attention::launch_decode(a, (int)head_dim, c.grid, st));
   if (!c.direct) KVOFF_TRY(attention::launch_join(a, (int)head_dim, c.grid, st));
   return ok();
+}
+
+extern "C" int kvoff_attention_fp8_packed(const int64_t* a) {
+  if (a == nullptr) return fail(KVOFF_EINVAL, "kvoff_attention_fp8_packed: null pointer");
+  double softmax_scale;
+  memcpy(&softmax_scale, a + 24, sizeof(softmax_scale));
+  return kvoff_attention_fp8(
+      reinterpret_cast<const void*>(a[0]), a[1], reinterpret_cast<void*>(a[2]), a[3],
+      reinterpret_cast<float*>(a[4]), reinterpret_cast<const void*>(a[5]),
+      reinterpret_cast<const void*>(a[6]), reinterpret_cast<const float*>(a[7]),
+      reinterpret_cast<const float*>(a[8]), a[9], a[10], a[11],
+      reinterpret_cast<const int32_t*>(a[12]), a[13], a[14], reinterpret_cast<const int32_t*>(a[15]),
+      reinterpret_cast<const int32_t*>(a[16]), a[17], a[18], a[19], a[20], a[21], a[22],
+      (int32_t)a[23], (float)softmax_scale, reinterpret_cast<void*>(a[25]), a[26],
+      reinterpret_cast<void*>(a[27]));
 }

@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "runtime.h"
 
 namespace kvoff {
@@ -299,6 +301,19 @@ constexpr int kExtendRows = 256;
 // short sequences ends last (64 sequences of 0 to 8192 keys: 243 us against 49).
 constexpr int kDecodeFixed = 768;
 constexpr int kExtendFixed = 512;
+// Raises a kernel's shared memory limit, once per kernel and device.
+template <void (*kKernel)(Args)>
+int allow_shared(int bytes) {
+  static std::atomic<uint64_t> done{0};  // one for each kernel: bit d is device d
+  int device = 0;
+  KVOFF_TRY(cuda_status(cudaGetDevice(&device), "cudaGetDevice"));
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if ((done.load(std::memory_order_relaxed) & bit) != 0) return KVOFF_OK;
+  KVOFF_TRY(cuda_status(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes),
+                        "attention_fp8 shared memory"));
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return KVOFF_OK;
+}
 int launch_decode(const Args& a, int dim, int grid, cudaStream_t stream);
 int launch_extend(const Args& a, int dim, int grid, cudaStream_t stream);
 

@@ -331,3 +331,13 @@ extern "C" int kvoff_rotary(const void* q, int64_t q_stride_bytes, void* q_out,
   if (rc != KVOFF_OK) return rc;
   return ok();
 }
+
+extern "C" int kvoff_rotary_packed(const int64_t* a) {
+  if (a == nullptr) return fail(KVOFF_EINVAL, "kvoff_rotary_packed: null pointer");
+  return kvoff_rotary(reinterpret_cast<const void*>(a[0]), a[1], reinterpret_cast<void*>(a[2]), a[3],
+                      a[4], reinterpret_cast<const void*>(a[5]), a[6], reinterpret_cast<void*>(a[7]),
+                      a[8], a[9], a[10], a[11], (int32_t)a[12], reinterpret_cast<const void*>(a[13]),
+                      (int32_t)a[14], reinterpret_cast<const float*>(a[15]), a[16], a[17],
+                      (int32_t)a[18], reinterpret_cast<int32_t*>(a[19]),
+                      reinterpret_cast<void*>(a[20]));
+}

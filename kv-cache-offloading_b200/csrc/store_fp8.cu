@@ -445,3 +445,13 @@ extern "C" int kvoff_store_kvcache_fp8(const void* key, int64_t key_stride_bytes
   if (rc != KVOFF_OK) return rc;
   return ok();
 }
+
+extern "C" int kvoff_store_kvcache_fp8_packed(const int64_t* a) {
+  if (a == nullptr) return fail(KVOFF_EINVAL, "kvoff_store_kvcache_fp8_packed: null pointer");
+  return kvoff_store_kvcache_fp8(
+      reinterpret_cast<const void*>(a[0]), a[1], reinterpret_cast<const void*>(a[2]), a[3],
+      reinterpret_cast<void*>(a[4]), reinterpret_cast<void*>(a[5]), reinterpret_cast<float*>(a[6]),
+      reinterpret_cast<float*>(a[7]), a[8], a[9], (int32_t)a[10], a[11],
+      reinterpret_cast<const int32_t*>(a[12]), a[13], a[14], reinterpret_cast<int32_t*>(a[15]),
+      reinterpret_cast<void*>(a[16]));
+}

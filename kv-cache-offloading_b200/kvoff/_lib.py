@@ -67,6 +67,9 @@ SIGNATURES = {
                                            _I64, _I32, ctypes.c_float, _P, _I64, _P]),
     "kvoff_attention_fp8_workspace": (ctypes.c_int, [_I64, _I64, _I64, _I64, _I64, _I64, _I64,
                                                      _PI64]),
+    "kvoff_rotary_packed": (ctypes.c_int, [ctypes.c_char_p]),
+    "kvoff_store_kvcache_fp8_packed": (ctypes.c_int, [ctypes.c_char_p]),
+    "kvoff_attention_fp8_packed": (ctypes.c_int, [ctypes.c_char_p]),
     "kvoff_host_alloc": (ctypes.c_int, [ctypes.c_uint64, _I32, _PP, _PP]),
     "kvoff_host_free": (ctypes.c_int, [_P]),
     "kvoff_device_numa_node": (ctypes.c_int, [_I32, ctypes.POINTER(_I32)]),

@@ -83,6 +83,17 @@ def test_empty_calls_are_accepted_without_a_device():
     assert attention(seqs=0, n=0, q=None) == _lib.KVOFF_OK
 
 
+@pytest.mark.parametrize("name,args", [("rotary", 21), ("store_kvcache_fp8", 17), ("attention_fp8", 28)])
+def test_packed_forms_reach_the_same_checks(name, args):
+    packed = getattr(_lib.lib(), f"kvoff_{name}_packed")
+    assert packed(None) == _lib.KVOFF_EINVAL and "null" in _lib.last_error()
+    values = (ctypes.c_int64 * args)(*([-1] * args))
+    assert packed(ctypes.cast(values, ctypes.c_char_p)) == _lib.KVOFF_EINVAL
+    assert f"kvoff_{name}: bad sizes" in _lib.last_error()
+    _lib.debug_fail_next(name)
+    assert packed(ctypes.cast(values, ctypes.c_char_p)) == _lib.KVOFF_EINJECTED
+
+
 @pytest.mark.parametrize("op,fn", [("rotary", rotary), ("store_kvcache_fp8", store), ("attention_fp8", attention)])
 def test_injected_failures(op, fn):
     _lib.debug_fail_next(op)
