@@ -60,14 +60,16 @@ __device__ __forceinline__ uint32_t smem_of(const void* p) {
 }
 
 template <int kBytes>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool real) {
-  const int size = real ? kBytes : 0;  // the rest is filled with zeros
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
   if (kBytes == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(size)
-                 : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
   else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(size)
-                 : "memory");
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+// 16 bytes, or zeros without a look at src.
+__device__ __forceinline__ void copy_async_or_zero(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0)
+               : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -310,63 +312,81 @@ __global__ void __launch_bounds__(kThreads, 2) attention_decode_fp8_kernel(const
     const int fewest = max(0, seq.context - seq.q_len + seg.tile * a.rows / a.group + 1);
     const int32_t* table = a.tables + seg.seq * a.table_stride;
     const int count = seg.end - seg.begin;
+    // This lane's 16-byte chunk of rows row0, row0 + kRowStep, ... of a tile.
+    constexpr int kRowStep = 32 / (D / 16), kCopies = kTile / kRowStep;
+    const int row0 = lane / (D / 16), chunk0 = lane % (D / 16);
+    const int64_t mine = row0 * row_bytes + seg.head * D + chunk0 * 16;
+    const uint8_t* k_from = a.cache[0] + mine;
+    const uint8_t* v_from = a.cache[1] + mine;
+    const float* scale_from = (lane == 0 ? a.scale[0] : a.scale[1]) + seg.head;
 
-    // Page ids of this warp's tiles, 32 at a time: lane i has tile i's.
-    auto page_of = [&](int i) {
+    // Where this warp's tiles stand, 32 at a time: lane i has tile i's first byte
+    // in the cache (at this head; negative: no page) and its scale's index. The
+    // divisions are made once for each tile here, not by every lane in the loop.
+    const int blocks = page_tiles / a.block_tiles;  // scale blocks of a page
+    int64_t place = -1, place_next = -1;
+    int32_t block = 0, block_next = 0;
+    auto look_up = [&](int i, int64_t& at, int32_t& scale) {
       const int tile = (seg.begin + i) * kWarps + warp;
-      int id = -1;
+      at = -1;
       if (i < count && tile * kTile < keys) {
-        id = __ldg(table + tile / page_tiles);
-        if (id >= a.num_pages) id = -1;
+        const int index = tile / page_tiles, in_page = tile - index * page_tiles;
+        const int id = __ldg(table + index);
+        if (id >= 0 && id < a.num_pages) {
+          at = ((int64_t)id * a.page + in_page * kTile) * row_bytes;
+          scale = id * blocks + in_page / a.block_tiles;
+        }
       }
-      return id;
     };
-    int pages = page_of(lane), pages_next = -1;
+    look_up(lane, place, block);
     uint32_t absent = 0;  // bit k: the tile issued k tiles ago has no page
 
-    auto issue = [&](int i) {
+    auto issue = [&](int i, int slot) {
       if (i < count) {
-        if (i > 0 && i % 32 == 0) pages = pages_next;
-        if (i % 32 == 8) pages_next = page_of(i - 8 + 32 + lane);
-        const int id = __shfl_sync(0xFFFFFFFFu, pages, i % 32);
-        const int tile = (seg.begin + i) * kWarps + warp;
-        const bool there = id >= 0;
-        absent = absent << 1 | (there ? 0u : 1u);
-        if (tile * kTile < keys) {
-          const int64_t page = there ? id : 0;
-          const int in_page = tile % page_tiles;
-          const uint32_t stage = ring + i % S::kStages * S::kStageBytes;
-          const int64_t at = (page * a.page + in_page * kTile) * row_bytes + seg.head * D;
-          constexpr int kChunks = D / 16;
+        if (i > 0 && i % 32 == 0) place = place_next, block = block_next;
+        if (i % 32 == 8) look_up(i - 8 + 32 + lane, place_next, block_next);
+        const int64_t at = __shfl_sync(0xFFFFFFFFu, place, i % 32);
+        const int32_t scale = __shfl_sync(0xFFFFFFFFu, block, i % 32);
+        const int left = keys - ((seg.begin + i) * kWarps + warp) * kTile;  // keys of the tile that are read
+        absent = absent << 1 | (at < 0 ? 1u : 0u);
+        const uint32_t stage = ring + slot * S::kStageBytes;
+        if (at >= 0 && left >= kTile) {
+          const uint8_t* k = k_from + at;
+          const uint8_t* v = v_from + at;
 #pragma unroll
-          for (int c = 0; c < kTile * kChunks / 32; ++c) {
-            const int id16 = lane + 32 * c, row = id16 / kChunks, chunk = id16 % kChunks;
-            const bool real = there && tile * kTile + row < keys;
-            const int64_t from = at + row * row_bytes + chunk * 16;
-            copy_async<16>(stage + k_place<D>(row, chunk), a.cache[0] + from, real);
-            copy_async<16>(stage + S::kTileBytes + v_place<D>(row, chunk), a.cache[1] + from, real);
+          for (int c = 0; c < kCopies; ++c) {
+            copy_async<16>(stage + k_place<D>(row0 + kRowStep * c, chunk0), k);
+            copy_async<16>(stage + S::kTileBytes + v_place<D>(row0 + kRowStep * c, chunk0), v);
+            k += kRowStep * row_bytes;
+            v += kRowStep * row_bytes;
           }
-          if (lane < 2) {
-            const int64_t block = page * (page_tiles / a.block_tiles) + in_page / a.block_tiles;
-            copy_async<4>(stage + 2 * S::kTileBytes + 4 * lane,
-                          (lane == 0 ? a.scale[0] : a.scale[1]) + block * a.kv_heads + seg.head, there);
+        } else if (at >= 0) {
+#pragma unroll
+          for (int c = 0; c < kCopies; ++c) {
+            const bool real = row0 + kRowStep * c < left;
+            const int64_t from = at + c * kRowStep * row_bytes;
+            copy_async_or_zero(stage + k_place<D>(row0 + kRowStep * c, chunk0), k_from + from, real);
+            copy_async_or_zero(stage + S::kTileBytes + v_place<D>(row0 + kRowStep * c, chunk0), v_from + from, real);
           }
         }
+        if (lane < 2 && at >= 0)
+          copy_async<4>(stage + 2 * S::kTileBytes + 4 * lane, scale_from + (int64_t)scale * a.kv_heads);
       }
       copy_commit();
     };
 
+    int stage_now = 0;
 #pragma unroll
-    for (int i = 0; i < S::kStages - 1; ++i) issue(i);
+    for (int i = 0; i < S::kStages - 1; ++i) issue(i, i);
 
     for (int i = 0; i < count; ++i) {
-      issue(i + S::kStages - 1);
+      issue(i + S::kStages - 1, stage_now == 0 ? S::kStages - 1 : stage_now - 1);
       copy_wait<S::kStages - 1>();
       __syncwarp();
       const int tile = (seg.begin + i) * kWarps + warp;
       const int behind = min(S::kStages - 1, count - 1 - i);  // tiles issued after this one
       if (tile * kTile < keys && (absent >> behind & 1) == 0) {
-        const uint32_t stage = ring + i % S::kStages * S::kStageBytes;
+        const uint32_t stage = ring + stage_now * S::kStageBytes;
         const float2 scales = load_shared_f2(stage + 2 * S::kTileBytes);
         float x[NT][4];
 #pragma unroll
@@ -473,6 +493,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_decode_fp8_kernel(const
           }
         }
       }
+      stage_now = stage_now == S::kStages - 1 ? 0 : stage_now + 1;
       __syncwarp();  // the stage is read before it is filled again
     }
     copy_wait<0>();

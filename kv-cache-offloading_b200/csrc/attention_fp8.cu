@@ -13,7 +13,8 @@ constexpr int kJoinThreads = 256;
 // Every record's CTA joins the split row tile that begins in that CTA of the
 // attention kernel: o = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c over its
 // parts, in the order of their keys, so the result does not depend on timing.
-// A warp takes a row; blockIdx.y picks 64 values of it.
+// A warp takes a row and blockIdx.y 64 values of it; lane i looks at part i, so
+// that the parts' maxima and then their sums are read side by side.
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Args a, int dim) {
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the parts are complete
   const int first = blockIdx.x;
@@ -24,30 +25,50 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   const int rows = min(a.rows, seq.q_len * a.group - record.tile * a.rows);
   const int lane = threadIdx.x % 32, d = blockIdx.y * 64 + lane * 2;
   const int64_t slot = slot_floats(a.rows, dim);
+  const float none = __int_as_float(0xFF800000);
   for (int row = threadIdx.x / 32 + blockIdx.z * (kJoinThreads / 32); row < rows;
        row += kJoinThreads / 32 * gridDim.z) {
-    float most = __int_as_float(0xFF800000), l = 0.0f;
+    float most = none, l = 0.0f;
     float2 sum = make_float2(0.0f, 0.0f);
     bool any = false;
-    auto part = [&](int cta, int which) {
-      const float* p = a.partial + ((int64_t)cta * 2 + which) * slot;
-      const float m = p[a.rows * dim + row], part_l = p[a.rows * dim + a.rows + row];
-      const float2 x = *reinterpret_cast<const float2*>(p + row * dim + d);
-      any = true;
-      const float top = fmaxf(most, m);
-      if (top == __int_as_float(0xFF800000)) {  // no key seen: o is 0, or NaN from NaN scores
-        sum.x += x.x, sum.y += x.y, l += part_l;
-        return;
-      }
-      const float keep = exp2_fast(most - top), take = exp2_fast(m - top);
-      sum.x = sum.x * keep + x.x * take;
-      sum.y = sum.y * keep + x.y * take;
-      l = l * keep + part_l * take;
+    for (int base = 0; base <= record.further; base += 32) {
+      // Part 0 is the CTA's own (slot 1), part i continues it in CTA first + i * stride.
+      const int part = base + lane, cta = first + part * a.stride;
+      bool valid = false;
+      if (part <= record.further) valid = part == 0 ? record.valid[1] != 0 : a.records[cta].valid[0] != 0;
+      const float* p = a.partial + ((int64_t)cta * 2 + (part == 0 ? 1 : 0)) * slot;
+      const float m = valid ? p[a.rows * dim + row] : none;
+      const float part_l = valid ? p[a.rows * dim + a.rows + row] : 0.0f;
+      float top = m;
+#pragma unroll
+      for (int k = 16; k > 0; k /= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, k));
+      top = fmaxf(top, most);
+      // Without a key seen the sums are 0, or NaN from NaN scores: they are added.
+      const float take = valid ? (top == none ? 1.0f : exp2_fast(m - top)) : 0.0f;
+      const float keep = top == none || most == top ? 1.0f : exp2_fast(most - top);
+      float add = take * part_l;
+      if (!valid) add = 0.0f;
+#pragma unroll
+      for (int k = 16; k > 0; k /= 2) add += __shfl_xor_sync(0xFFFFFFFFu, add, k);
+      l = l * keep + add;
+      sum.x *= keep;
+      sum.y *= keep;
       most = top;
-    };
-    if (record.valid[1]) part(first, 1);
-    for (int c = first + 1; c <= first + record.further; ++c)
-      if (a.records[c].valid[0]) part(c, 0);
+      const uint32_t mask = __ballot_sync(0xFFFFFFFFu, valid);
+      any = any || mask != 0;
+      const int last = min(31, record.further - base);
+#pragma unroll 8
+      for (int i = 0; i <= last; ++i) {
+        const float weight = __shfl_sync(0xFFFFFFFFu, take, i);
+        if ((mask >> i & 1) != 0) {
+          const int from = first + (base + i) * a.stride;
+          const float2 x = *reinterpret_cast<const float2*>(
+              a.partial + ((int64_t)from * 2 + (base + i == 0 ? 1 : 0)) * slot + row * dim + d);
+          sum.x += weight * x.x;
+          sum.y += weight * x.y;
+        }
+      }
+    }
     if (!any) continue;  // one CTA had all of it and wrote the result
     const int at = record.tile * a.rows + row;
     const int token = seq.start + at / a.group, head = record.head * a.group + at % a.group;
@@ -84,7 +105,7 @@ struct Shape {
 
 // How a call is launched: rows of a tile, CTAs, and whether rows are split.
 struct Choice {
-  int rows, grid;
+  int rows, grid, stride;
   int64_t max_tiles;
   bool direct, extend;
 };
@@ -97,7 +118,9 @@ Choice choose(const Shape& s) {
   c.max_tiles = (rows + c.rows - 1) / c.rows;
   const int64_t ctas = s.seqs * s.kv_heads * c.max_tiles;
   c.direct = s.keys <= kDirectKeys && ctas <= 0x7FFFFFFFll;
-  c.grid = c.direct ? (int)ctas : c.extend ? sm_count() : 2 * sm_count();
+  c.stride = c.extend ? 1 : (int)s.kv_heads;
+  const int parts = 2 * sm_count() / (int)s.kv_heads;  // of a head's work
+  c.grid = c.direct ? (int)ctas : c.extend ? sm_count() : (parts > 1 ? parts : 1) * c.stride;
   return c;
 }
 
@@ -217,6 +240,7 @@ extern "C" int kvoff_attention_fp8(
   a.fixed = c.extend ? attention::kExtendFixed : attention::kDecodeFixed;
   a.max_tiles = (int32_t)c.max_tiles;
   a.direct = c.direct;
+  a.stride = c.stride;
   a.bf16 = dtype == KVOFF_BF16;
   a.wide_out = (pairs & 15u) == 0;
   a.records = static_cast<attention::Record*>(workspace);

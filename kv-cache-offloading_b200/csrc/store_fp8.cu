@@ -48,10 +48,6 @@
 namespace kvoff {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kKeptLarge = 8;   // rows of a thread group held in registers between the passes
-constexpr int kKeptSmall = 4;
-constexpr int kResident = 2;    // CTAs an SM: registers for the rows that are held
 constexpr int kWindow = 16;     // tokens a CTA looks at for the start of a run
 constexpr int64_t kSmallCall = 1024;  // up to here a CTA looks at one token
 constexpr int64_t kMostTokens = 65536;
@@ -148,7 +144,6 @@ __device__ __forceinline__ uint2 rescale(const uint2& payload, float factor) {
   return out;
 }
 
-template <typename T>
 __device__ __forceinline__ uint4 load_row(const uint8_t* p) {
   uint4 v;  // read once: kept out of L1, which holds the slots
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
@@ -157,15 +152,15 @@ __device__ __forceinline__ uint4 load_row(const uint8_t* p) {
   return v;
 }
 
-template <typename T, int LANES, int kKept>
-__global__ void __launch_bounds__(kThreads, kResident)
+template <typename T, int LANES, int THREADS, int KEPT>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
     store_kvcache_fp8_kernel(const __grid_constant__ StoreArgs a) {
-  constexpr int kGroups = kThreads / LANES;
+  constexpr int kGroups = THREADS / LANES;
   extern __shared__ int32_t winner[];  // last token that writes each row of the block, or -1
   __shared__ int32_t window[kWindow];
   __shared__ uint32_t starts;
   __shared__ uint32_t amax[kGroups];
-  __shared__ int32_t earlier, far;
+  __shared__ int32_t earlier, last;
   const int tid = threadIdx.x;
   const int first = blockIdx.x * a.window;
 
@@ -185,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, kResident)
     const int32_t previous = __shfl_sync(0xFFFFFFFFu, id, before == 0 ? 0 : 31 - __clz(before));
     const bool start = own && id >= 0 && (before == 0 || previous != id);
     const uint32_t mask = __ballot_sync(0xFFFFFFFFu, start) >> (32 - kWindow);
-    if (own) window[tid - (32 - kWindow)] = id;
+    if (own) window[tid - (32 - kWindow)] = slot;
     if (tid == 0) starts = mask;
   }
   __syncthreads();
@@ -206,44 +201,38 @@ __global__ void __launch_bounds__(kThreads, kResident)
       (is_v ? a.rows[1] : a.rows[0]) + ((int64_t)head * a.dim + lane * 8) * sizeof(T);
   for (; todo != 0; todo &= todo - 1) {
     const int w = __ffs(todo) - 1, leader = first + w;
-    const int32_t id = window[w];
-    for (int i = tid; i < (int)block; i += kThreads) winner[i] = -1;
+    const int32_t id = window[w] >> a.shift, base = id << a.shift;
+    const int32_t begin = window[w] - base;  // the leader's row
+    for (int i = tid; i < (int)block; i += THREADS) winner[i] = -1;
     if (tid < a.pairs) amax[tid] = 0;
-    if (tid == 0) earlier = far = 0;
+    if (tid == 0) earlier = last = 0;
+    // Rows that are nearly always the block's are on the way while the slots are
+    // looked at: those of the tokens after the leader in a large call, which
+    // holds prompts; the leader's own in a small one.
+    const uint8_t* run = source + (leader + sub) * stride;
+    const int likely = a.window > 1 ? min((int)block - begin, a.num_tokens - leader) : 1;
+    uint4 kept[KEPT];
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i)
+      if (active && sub + i * subs < likely) kept[i] = load_row(run + i * subs * stride);
+    float* scale = (is_v ? a.scale[1] : a.scale[0]) + (int64_t)id * a.heads + head;
+    float before = 0.0f;
+    if (active) before = *scale;
     __syncthreads();
-    const int32_t base = id << a.shift;
     // A slot's row in the block, or a number not below `block`.
     auto row_of = [&](int32_t slot) { return (uint32_t)slot - (uint32_t)base; };
-    // The rows of the run, which are nearly always all of the block's: this
-    // thread's are on the way while the other slots are looked at.
-    uint4 kept[kKept];
-    int32_t offset[kKept];
-#pragma unroll
-    for (int i = 0; i < kKept; ++i) {
-      const int r = sub + i * subs, token = leader + r;
-      offset[i] = -1;
-      if (r < (int)block && token < a.num_tokens) {
-        const uint32_t row = row_of(__ldg(a.slots + token));
-        if (row < block) {
-          offset[i] = (int32_t)row;
-          if (active) kept[i] = load_row<T>(source + token * stride);
-        }
-      }
-    }
     auto look = [&](int i, int32_t slot) {
       if (row_of(slot) < block) {
-        if (i < leader) {
+        if (i < leader)
           earlier = 1;
-        } else {
+        else
           atomicMax(&winner[row_of(slot)], i);
-          if (i >= leader + (int)block) far = 1;
-        }
       }
     };
     if (a.wide_slots) {
       const int quads = a.num_tokens / 4;
 #pragma unroll 4
-      for (int i = tid; i < quads; i += kThreads) {
+      for (int i = tid; i < quads; i += THREADS) {
         const int4 s = __ldg(reinterpret_cast<const int4*>(a.slots) + i);
         if (min(min(row_of(s.x), row_of(s.y)), min(row_of(s.z), row_of(s.w))) < block) {
           look(4 * i, s.x);
@@ -252,50 +241,46 @@ __global__ void __launch_bounds__(kThreads, kResident)
           look(4 * i + 3, s.w);
         }
       }
-      for (int i = 4 * quads + tid; i < a.num_tokens; i += kThreads) look(i, __ldg(a.slots + i));
+      for (int i = 4 * quads + tid; i < a.num_tokens; i += THREADS) look(i, __ldg(a.slots + i));
     } else {
-      for (int i = tid; i < a.num_tokens; i += kThreads) look(i, __ldg(a.slots + i));
+      for (int i = tid; i < a.num_tokens; i += THREADS) look(i, __ldg(a.slots + i));
     }
-    float* scale = (is_v ? a.scale[1] : a.scale[0]) + (int64_t)id * a.heads + head;
-    float before = 0.0f;
-    if (active) before = *scale;
     __syncthreads();
     if (earlier != 0) {  // another CTA owns the block
       __syncthreads();
       continue;
     }
+    // The usual case: tokens that follow one another write rows that follow one
+    // another (some may be skipped), up to `extent` of them from `begin` on, and no
+    // other token writes here.
+    bool in_order = true;
+    int most_row = 0;
+    for (int i = tid; i < (int)block; i += THREADS)
+      if (winner[i] >= 0) {
+        in_order = in_order && winner[i] - leader == i - begin;
+        most_row = i + 1;
+      }
+    most_row = __reduce_max_sync(0xFFFFFFFFu, most_row);
+    if (tid % 32 == 0 && most_row > 0) atomicMax(&last, most_row);
+    const bool regular = __syncthreads_and(in_order);
+    const int extent = last - begin;
     const bool opened = winner[0] >= 0;
     const float old =
         !opened && before > 0.0f && __float_as_uint(before) < 0x7F800000u ? before : 0.0f;
 
     uint8_t* target = (is_v ? a.cache[1] : a.cache[0]) + base * row_bytes +
                       (int64_t)head * a.dim + lane * 8;
-    // Calls f(row, offset) for this thread's rows that are not in `kept`: the
-    // rest of the run, and rows of the block from further on in the call.
+    // Calls f(row, its number in the block) for this thread's rows that are not
+    // in `kept`.
     auto others = [&](auto f) {
-      constexpr int kBatch = 4;  // loads in flight
-      for (int r = sub + kKept * subs; r < (int)block; r += kBatch * subs) {
-        uint4 row[kBatch];
-        int at[kBatch];
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int token = leader + r + i * subs;
-          at[i] = -1;
-          if (r + i * subs < (int)block && token < a.num_tokens) {
-            const uint32_t to = row_of(__ldg(a.slots + token));
-            if (to < block && winner[to] == token) {
-              at[i] = (int)to;
-              row[i] = load_row<T>(source + token * stride);
-            }
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i)
-          if (at[i] >= 0) f(row[i], at[i]);
-      }
-      if (far != 0)
+      if (regular) {
+#pragma unroll 4
+        for (int r = sub + KEPT * subs; r < extent; r += subs)
+          if (winner[begin + r] >= 0) f(load_row(source + (leader + r) * stride), begin + r);
+      } else {
         for (int r = sub; r < (int)block; r += subs)
-          if (winner[r] >= leader + (int)block) f(load_row<T>(source + winner[r] * stride), r);
+          if (winner[r] >= 0) f(load_row(source + winner[r] * stride), r);
+      }
     };
     uint32_t most = 0;
     bool finite = true;
@@ -305,14 +290,19 @@ __global__ void __launch_bounds__(kThreads, kResident)
       finite = false;
       return largest_finite<T>(row);
     };
+    uint32_t held = 0;  // bit i: kept[i] is written
     if (active) {
 #pragma unroll
-      for (int i = 0; i < kKept; ++i) {
-        if (offset[i] >= 0 && winner[offset[i]] != leader + sub + i * subs) offset[i] = -1;
-        if (offset[i] >= 0) {
-          most = max(most, size_of(kept[i]));
+      for (int i = 0; i < KEPT; ++i) {
+        const int r = sub + i * subs;
+        if (regular && r < extent && winner[begin + r] >= 0) {
+          held |= 1u << i;
+          if (r >= likely) kept[i] = load_row(run + i * subs * stride);
         }
       }
+#pragma unroll
+      for (int i = 0; i < KEPT; ++i)
+        if (held >> i & 1) most = max(most, size_of(kept[i]));
       others([&](const uint4& row, int) { most = max(most, size_of(row)); });
     }
 #pragma unroll
@@ -323,14 +313,16 @@ __global__ void __launch_bounds__(kThreads, kResident)
       const float now = fmaxf(scale_for<T>(amax[mine]), old);
       const float reciprocal = __fdiv_rn(1.0f, now);
       const bool plain = finite && (__float_as_uint(now) & 0x7FFFFFu) == 0;
-      auto put = [&](const uint4& row, int at) {
-        *reinterpret_cast<uint2*>(target + at * row_bytes) =
-            plain ? encode_finite<T>(row, reciprocal) : encode_any<T>(row, now);
+      auto put = [&](const uint4& row, uint8_t* to) {
+        *reinterpret_cast<uint2*>(to) = plain ? encode_finite<T>(row, reciprocal) : encode_any<T>(row, now);
       };
+      uint8_t* to = target + (begin + sub) * row_bytes;
 #pragma unroll
-      for (int i = 0; i < kKept; ++i)
-        if (offset[i] >= 0) put(kept[i], offset[i]);
-      others(put);
+      for (int i = 0; i < KEPT; ++i) {
+        if (held >> i & 1) put(kept[i], to);
+        to += subs * row_bytes;
+      }
+      others([&](const uint4& row, int at) { put(row, target + at * row_bytes); });
       if (!opened && now != old) {
         const float factor = __fdiv_rn(old, now);
         for (int r = sub; r < (int)block; r += subs)
@@ -345,40 +337,43 @@ __global__ void __launch_bounds__(kThreads, kResident)
   }
 }
 
-template <typename T, int LANES, int kKept>
+template <typename T, int LANES, int THREADS, int KEPT>
 int launch(StoreArgs a, cudaStream_t stream) {
-  constexpr int kGroups = kThreads / LANES;
+  constexpr int kGroups = THREADS / LANES;
   const int block = 1 << a.shift;
   a.window = a.num_tokens <= kSmallCall ? 1 : kWindow;
-  // As many pairs a CTA as it has thread groups, fewer while that leaves SMs
-  // without a block (a prompt of one sequence in long blocks).
+  // As many pairs a CTA as it has thread groups; fewer while that leaves SMs
+  // without a block (a prompt of one sequence in long blocks), or while a group
+  // has more rows than it holds in registers.
   const int64_t blocks = a.num_tokens <= kSmallCall && a.num_tokens < block
                              ? a.num_tokens
                              : (a.num_tokens + block - 1) / block;
   int pairs = 1;
   while (pairs < kGroups && pairs < 2 * a.heads) pairs *= 2;
-  while (pairs > 1 && blocks * ((2 * a.heads + pairs - 1) / pairs) < 2 * sm_count()) pairs /= 2;
-  while (pairs > 1 && kGroups / pairs * kKept < block) pairs /= 2;
+  while (pairs > 1 && (blocks * ((2 * a.heads + pairs - 1) / pairs) < sm_count() ||
+                       kGroups / pairs * KEPT < (a.window > 1 ? block : 1)))
+    pairs /= 2;
   a.pairs = pairs;
   while ((1 << a.pair_shift) < pairs) ++a.pair_shift;
   const dim3 grid((a.num_tokens + a.window - 1) / a.window, (2 * a.heads + pairs - 1) / pairs);
-  store_kvcache_fp8_kernel<T, LANES, kKept>
-      <<<grid, kThreads, block * sizeof(int32_t), stream>>>(a);
+  store_kvcache_fp8_kernel<T, LANES, THREADS, KEPT>
+      <<<grid, THREADS, block * sizeof(int32_t), stream>>>(a);
   return cuda_status(cudaGetLastError(), "store_kvcache_fp8 launch");
 }
 
 template <typename T, int LANES>
-int launch_kept(const StoreArgs& a, cudaStream_t stream) {
-  return a.num_tokens <= kSmallCall ? launch<T, LANES, kKeptSmall>(a, stream) : launch<T, LANES, kKeptLarge>(a, stream);
+int launch_size(const StoreArgs& a, cudaStream_t stream) {
+  return a.num_tokens <= kSmallCall ? launch<T, LANES, 256, 4>(a, stream)
+                                    : launch<T, LANES, 512, 4>(a, stream);
 }
 
 template <typename T>
 int launch_lanes(const StoreArgs& a, cudaStream_t stream) {
   const int vectors = a.dim / 8;
-  if (vectors <= 4) return launch_kept<T, 4>(a, stream);
-  if (vectors <= 8) return launch_kept<T, 8>(a, stream);
-  if (vectors <= 16) return launch_kept<T, 16>(a, stream);
-  return launch_kept<T, 32>(a, stream);
+  if (vectors <= 4) return launch_size<T, 4>(a, stream);
+  if (vectors <= 8) return launch_size<T, 8>(a, stream);
+  if (vectors <= 16) return launch_size<T, 16>(a, stream);
+  return launch_size<T, 32>(a, stream);
 }
 
 }  // namespace
