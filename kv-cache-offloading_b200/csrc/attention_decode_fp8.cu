@@ -305,8 +305,6 @@ __global__ void __launch_bounds__(kThreads, 2) attention_decode_fp8_kernel(const
   Segment seg;
   while (walk.next(a, &seg)) {
     const Sequence& seq = walk.seq;
-    Rows<D, NT> r;
-    load_rows<D, NT>(a, seq, seg, g, t, r);
     const int keys = min(seq.keys(a, seg.tile), seq.context);  // that any row sees
     // The fewest keys that a row sees: tiles below it need no mask.
     const int fewest = max(0, seq.context - seq.q_len + seg.tile * a.rows / a.group + 1);
@@ -376,8 +374,10 @@ __global__ void __launch_bounds__(kThreads, 2) attention_decode_fp8_kernel(const
     };
 
     int stage_now = 0;
-#pragma unroll
+#pragma unroll 1  // code that runs once is fetched cold: the less of it the better
     for (int i = 0; i < S::kStages - 1; ++i) issue(i, i);
+    Rows<D, NT> r;  // while the first tiles are on their way
+    load_rows<D, NT>(a, seq, seg, g, t, r);
 
     for (int i = 0; i < count; ++i) {
       issue(i + S::kStages - 1, stage_now == 0 ? S::kStages - 1 : stage_now - 1);
@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_decode_fp8_kernel(const
               nan = nan || __vcmpeq4(v.w[k][n] & 0x7F7F7F7Fu, 0x7F7F7F7Fu) != 0;
           nan = __any_sync(0xFFFFFFFFu, nan);
         }
-        if (nan) {
+        if (__builtin_expect(nan, 0)) {
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
             bool see[4];
@@ -497,6 +497,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_decode_fp8_kernel(const
       __syncwarp();  // the stage is read before it is filled again
     }
     copy_wait<0>();
+    if (!a.direct) launch_dependents();
 
     // Join the warps: maxima first, then the sums at the common maximum.
 #pragma unroll

@@ -940,6 +940,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_extend_fp8_kernel(const
     }
     __syncwarp();
   }
+  if (!a.direct) launch_dependents();
   tensor_fence_before();
   __syncthreads();
   tensor_fence_after();

@@ -188,7 +188,7 @@ extern "C" int kvoff_attention_fp8(
     return fail(KVOFF_EINVAL, "kvoff_attention_fp8: q and out are bf16 or fp16");
   if (cu_seqlens_q == nullptr && (num_tokens != num_seqs || max_seqlen_q != 1))
     return fail(KVOFF_EINVAL, "kvoff_attention_fp8: without cu_seqlens_q each sequence has one token");
-  if (num_tokens > 0x7FFFFFFFll / q_heads)
+  if (num_tokens > 0x7FFFF000ll / q_heads)
     return fail(KVOFF_EINVAL, "kvoff_attention_fp8: sizes exceed 32 bits");
   if (!(softmax_scale > 0.0f && softmax_scale < 3.4e38f))
     return fail(KVOFF_EINVAL, "kvoff_attention_fp8: softmax_scale must be positive and finite");
@@ -237,6 +237,8 @@ extern "C" int kvoff_attention_fp8(
   a.kv_heads = (int32_t)kv_heads;
   a.group = (int32_t)(q_heads / kv_heads);
   a.rows = c.rows;
+  while ((1 << a.row_shift) < c.rows) ++a.row_shift;
+  a.tiles_per_cost = 1.0 / (attention::kKeyTile * (double)(q_heads / kv_heads));
   a.fixed = c.extend ? attention::kExtendFixed : attention::kDecodeFixed;
   a.max_tiles = (int32_t)c.max_tiles;
   a.direct = c.direct;

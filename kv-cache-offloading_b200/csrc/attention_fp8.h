@@ -32,7 +32,9 @@ struct Args {
   int32_t table_width, num_pages, page, block_tiles;  // scale block in 16-key units
   int32_t page_shift;  // log2 of page, or -1 when it is no power of two
   int32_t seqs, num_tokens, q_heads, kv_heads, group;
-  int32_t rows;      // packed rows of a row tile
+  int32_t rows;      // packed rows of a row tile: 2^row_shift
+  int32_t row_shift;
+  double tiles_per_cost;  // 1 / (kKeyTile * group)
   int32_t fixed;     // what beginning and ending a row tile costs, as keys read
   int32_t max_tiles; // row tiles of the longest sequence (direct form)
   bool direct;       // one CTA per (sequence, head, row tile), nothing is split
@@ -74,26 +76,24 @@ struct Sequence {
       start = min(max(a.starts[s], 0), a.num_tokens);
       q_len = min(max(a.starts[s + 1], start), a.num_tokens) - start;
     }
-    const int64_t room = (int64_t)a.table_width * a.page;
-    context = (int32_t)min((int64_t)max(a.contexts[s], 0), room);
-    const int64_t rows = (int64_t)q_len * a.group;
-    tiles = (int32_t)((rows + a.rows - 1) / a.rows);
+    context = min(max(a.contexts[s], 0), a.table_width * a.page);  // checked to fit 32 bits
+    tiles = (int32_t)(((uint32_t)(q_len * a.group) + a.rows - 1) >> a.row_shift);
     base = (int64_t)(max(context - q_len, 0) + a.fixed) * a.group;
   }
   __device__ __forceinline__ int64_t cost(const Args& a, int r) const {
-    return base + min((int64_t)(r + 1) * a.rows, (int64_t)q_len * a.group);
+    return base + min((r + 1) << a.row_shift, q_len * a.group);
   }
   // Cost of the row tiles before r (all of them whole).
   __device__ __forceinline__ int64_t before(const Args& a, int64_t r) const {
-    return r * base + a.rows * (r * (r + 1) / 2);
+    return r * base + ((r * (r + 1) / 2) << a.row_shift);
   }
   __device__ __forceinline__ int64_t per_head(const Args& a) const {
     return tiles == 0 ? 0 : before(a, tiles - 1) + cost(a, tiles - 1);
   }
   // Keys that the last row of tile r sees.
   __device__ __forceinline__ int keys(const Args& a, int r) const {
-    const int64_t last = min((int64_t)(r + 1) * a.rows, (int64_t)q_len * a.group) - 1;
-    return max(0, context - q_len + (int)(last / a.group) + 1);
+    const int last = min((r + 1) << a.row_shift, q_len * a.group) - 1;
+    return max(0, context - q_len + last / a.group + 1);
   }
 };
 
@@ -171,7 +171,7 @@ struct Walk {
     // A stretch of less than two key tiles costs more to join than to read.
     const int64_t least = (int64_t)(2 * kKeyTile + a.fixed) * a.group;
     const int parts = gridDim.x / a.stride;
-    share = max((total + parts - 1) / parts, least);
+    share = max((int64_t)((double)total / parts) + 1, least);
     from = cta / a.stride * share;
     to = min(from + share, total);
     more = from < to;
@@ -195,7 +195,9 @@ struct Walk {
     seq.load(a, s);
     const int64_t per_head = seq.per_head(a);
     if (a.stride == 1) {
-      head = (int)((from - at) / per_head);
+      head = (int)((double)(from - at) / (double)per_head);
+      while (head * per_head > from - at) --head;  // the quotient may be one off
+      while ((head + 1) * per_head <= from - at) ++head;
       at += head * per_head;
     } else {
       head = cta % a.stride;
@@ -216,7 +218,9 @@ struct Walk {
   __device__ __forceinline__ int cut(const Args& a, int64_t x, int64_t cost, int tiles) const {
     if (x >= at + cost) return tiles;
     const int64_t read = x - at - (int64_t)a.fixed * a.group;
-    return read <= 0 ? 0 : (int)min((int64_t)tiles, read / ((int64_t)kKeyTile * a.group));
+    // In doubles: 64-bit divisions are 100 instructions, and all that counts is that
+    // both sides of a cut get the same number.
+    return read <= 0 ? 0 : (int)min((double)tiles, (double)read * a.tiles_per_cost);
   }
 
   __device__ __forceinline__ void advance(const Args& a) {
@@ -260,7 +264,10 @@ struct Walk {
           record.seq = s;
           record.head = head;
           record.tile = tile;
-          record.further = (int32_t)((at + cost - 1) / share) - cta / a.stride;
+          // The CTA in whose stretch the triple's last unit lies.
+          int to_cta = cta / a.stride;
+          for (int64_t end_of = to; end_of < at + cost; end_of += share) ++to_cta;
+          record.further = to_cta - cta / a.stride;
         }
       } else {
         out->whole = true;
@@ -281,6 +288,9 @@ struct Walk {
 __host__ __device__ inline int64_t slot_floats(int rows, int dim) {
   return (int64_t)rows * (dim + 2);
 }
+
+// Lets the join be launched while this kernel ends; it waits for the results itself.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;"); }
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
