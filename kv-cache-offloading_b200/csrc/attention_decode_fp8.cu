@@ -47,11 +47,15 @@ constexpr float kWeight = 256.0f;   // of P in f16
 constexpr uint32_t kNegInf = 0xFF800000u;
 static_assert(kKeyTile == kWarps * kTile, "one tile a warp and key tile");
 
-template <int D>
+// One CTA an SM, eight warps with all the registers they can use. With two CTAs
+// at 128 registers (and half the stages each) 16 rows were spilled (138 us, now
+// 75: 4 x 34816 keys, 8 heads of 128, 12 rows) and 8 rows took 69 us, now 59. Two
+// tiles in one step take as long as one (60).
+template <int D, int NT>
 struct Shape {
   static constexpr int kTileBytes = kTile * D;             // of K, and of V
   static constexpr int kStageBytes = 2 * kTileBytes + 16;  // and the two scales
-  static constexpr int kStages = D == 64 ? 4 : 3;
+  static constexpr int kStages = D == 64 ? 8 : 6;
   static constexpr int kWarpBytes = kStages * kStageBytes;
 };
 
@@ -289,8 +293,8 @@ __device__ __forceinline__ void nan_tile(const VTile<D>& v, const uint32_t (&p)[
 }
 
 template <int D, int NT>
-__global__ void __launch_bounds__(kThreads, 2) attention_decode_fp8_kernel(const __grid_constant__ Args a) {
-  using S = Shape<D>;
+__global__ void __launch_bounds__(kThreads, 1) attention_decode_fp8_kernel(const __grid_constant__ Args a) {
+  using S = Shape<D, NT>;
   constexpr int kSteps = D / 16;
   constexpr int kRows = 8 * NT;
   extern __shared__ __align__(128) uint8_t shared[];
@@ -388,9 +392,11 @@ __global__ void __launch_bounds__(kThreads, 2) attention_decode_fp8_kernel(const
       if (tile * kTile < keys && (absent >> behind & 1) == 0) {
         const uint32_t stage = ring + stage_now * S::kStageBytes;
         const float2 scales = load_shared_f2(stage + 2 * S::kTileBytes);
-        float x[NT][4];
+        float x[NT][4], odd[NT][4];  // two chains of products, half as long
 #pragma unroll
-        for (int j = 0; j < NT; ++j) x[j][0] = x[j][1] = x[j][2] = x[j][3] = 0.0f;
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) x[j][k] = odd[j][k] = 0.0f;
 #pragma unroll
         for (int c = 0; c < D / 64; ++c) {
           const uint4 lo = load_shared16(stage + k_place<D>(g, 4 * c + t));
@@ -402,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_decode_fp8_kernel(const
             const uint32_t a2 = widen_high(low[k]), a3 = widen_high(high[k]);
 #pragma unroll
             for (int j = 0; j < NT; ++j)
-              mma(x[j], a0, a1, a2, a3, r.q[j][4 * c + k][0], r.q[j][4 * c + k][1]);
+              mma(k % 2 == 0 ? x[j] : odd[j], a0, a1, a2, a3, r.q[j][4 * c + k][0], r.q[j][4 * c + k][1]);
           }
         }
         VTile<D> v;
@@ -415,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_decode_fp8_kernel(const
         for (int j = 0; j < NT; ++j)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            x[j][k] *= scales.x * r.factor[j][k & 1];
+            x[j][k] = (x[j][k] + odd[j][k]) * (scales.x * r.factor[j][k & 1]);
             if (masked && tile * kTile + g + 8 * (k >> 1) >= r.limit[j][k & 1])
               x[j][k] = __uint_as_float(kNegInf);
             raise = raise || x[j][k] > r.m[j][k & 1] + kRaise;
@@ -575,10 +581,10 @@ __global__ void __launch_bounds__(kThreads, 2) attention_decode_fp8_kernel(const
 
 template <int D, int NT>
 int launch(const Args& a, int grid, cudaStream_t stream) {
-  constexpr int kRing = kWarps * Shape<D>::kWarpBytes;
+  constexpr int kRing = kWarps * Shape<D, NT>::kWarpBytes;
   constexpr int kSums = kWarps * 8 * NT * (D + 4) * (int)sizeof(float);
   constexpr int kBytes = kRing > kSums ? kRing : kSums;
-  static_assert(kBytes <= 112 * 1024, "two CTAs an SM");
+  static_assert(kBytes <= 224 * 1024, "shared memory");
   KVOFF_TRY((allow_shared<attention_decode_fp8_kernel<D, NT>>(kBytes)));
   attention_decode_fp8_kernel<D, NT><<<grid, kThreads, kBytes, stream>>>(a);
   return cuda_status(cudaGetLastError(), "attention_fp8 launch");

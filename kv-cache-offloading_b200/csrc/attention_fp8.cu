@@ -119,7 +119,7 @@ Choice choose(const Shape& s) {
   const int64_t ctas = s.seqs * s.kv_heads * c.max_tiles;
   c.direct = s.keys <= kDirectKeys && ctas <= 0x7FFFFFFFll;
   c.stride = c.extend ? 1 : (int)s.kv_heads;
-  const int parts = 2 * sm_count() / (int)s.kv_heads;  // of a head's work
+  const int parts = sm_count() / (int)s.kv_heads;  // of a head's work
   c.grid = c.direct ? (int)ctas : c.extend ? sm_count() : (parts > 1 ? parts : 1) * c.stride;
   return c;
 }
