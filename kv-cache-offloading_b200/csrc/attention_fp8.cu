@@ -113,7 +113,11 @@ struct Choice {
 Choice choose(const Shape& s) {
   Choice c{};
   const int64_t rows = s.max_q * (s.q_heads / s.kv_heads);
-  c.extend = rows > kDecodeRows;
+  // The decode kernel reads the cache once for 16 rows, the prompt kernel once
+  // for 256 and at the tensor cores' rate, but it takes longer to begin. Measured
+  // (8 heads of 128, us, decode kernel / prompt kernel): 24 rows of 34816 keys 49
+  // / 62, 32 rows 49 / 60, 64 rows 76 / 62; 64 rows of 300 keys 10.5 / 18.4.
+  c.extend = rows > (s.keys <= kDirectKeys ? 64 : 32);
   c.rows = c.extend ? kExtendRows : rows <= 8 ? 8 : kDecodeRows;
   c.max_tiles = (rows + c.rows - 1) / c.rows;
   const int64_t ctas = s.seqs * s.kv_heads * c.max_tiles;

@@ -108,8 +108,7 @@ struct Segment {
 // Deals the work of a launch over its CTAs. With stride kv_heads, CTA c has head
 // c % kv_heads, and the heads are dealt alike: CTAs that run side by side read
 // the same tokens' rows of all heads, which stand next to one another in memory
-// (decode of 4 x 34816 keys, 8 heads of 128: 72 us with the cuts of the heads
-// apart). With stride 1 the heads stand on the axis too. The key reads of all (sequence,
+// With stride 1 the heads stand on the axis too. The key reads of all (sequence,
 // head, row tile) triples, and a fixed cost of each, stand on one axis, in that order; each CTA takes an
 // equal stretch of it, cut at key tiles. So a batch of unequal lengths, or one
 // long sequence, keeps all SMs busy to the end, from lengths that only the
@@ -320,7 +319,7 @@ int launch_join(const Args& a, int dim, int grid, cudaStream_t stream);
 
 // The kernels. `dim` is 64 or 128; a is filled but for rows and partial.
 // Rows are packed rows of a KV head: query tokens times `group`.
-constexpr int kDecodeRows = 16;   // the most of one row tile
+constexpr int kDecodeRows = 16;   // the most of one row tile; 8 when no call has more
 constexpr int kExtendRows = 256;
 // Beginning and ending a row tile of a decode step takes 4.3 us, against 0.5
 // us a tile of 128 keys. Without it in the partition a CTA that gets a hundred
