@@ -321,9 +321,10 @@ int launch_join(const Args& a, int dim, int grid, cudaStream_t stream);
 // Rows are packed rows of a KV head: query tokens times `group`.
 constexpr int kDecodeRows = 16;   // the most of one row tile; 8 when no call has more
 constexpr int kExtendRows = 256;
-// Beginning and ending a row tile of a decode step takes 4.3 us, against 0.5
-// us a tile of 128 keys. Without it in the partition a CTA that gets a hundred
-// short sequences ends last (64 sequences of 0 to 8192 keys: 243 us against 49).
+// What beginning and ending a row tile costs, as keys read: 4 to 5 us of a decode
+// step, against 0.7 us a tile of 128 keys. Without it in the partition a CTA that
+// gets a hundred short sequences ends last (64 sequences of 0 to 8192 keys: 243
+// us; 512 keys 51, 768 keys 47, 1152 keys 52).
 constexpr int kDecodeFixed = 768;
 constexpr int kExtendFixed = 512;
 // Raises a kernel's shared memory limit, once per kernel and device.

@@ -18,7 +18,15 @@
 // unit in one thread a decode step of four tokens would use a few warps only,
 // and with one head per thread every thread would load more table than data,
 // so the heads are dealt over `lanes` threads: one head each while the grid
-// is small, four once the tokens alone fill the GPU.
+// is small, four once the tokens alone fill the GPU. The values are loaded
+// before the position is known, so one latency and not three stands between
+// them and the result.
+//
+// Measured: 16384 tokens, 64 + 8 heads of 128 bf16 in 93 us = 6.6 TB/s, a
+// copy's rate (197 us with the table row waited for first and two-byte
+// accesses to registers); 4096 tokens, 32 + 8 heads in 15.5 us; 4 tokens in
+// 2.1 us. Five heads a thread spill (30 us for the 4096 tokens), eight leave
+// too few threads (22 us).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
