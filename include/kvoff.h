@@ -74,7 +74,9 @@ KVOFF_API int kvoff_debug_fail_next(const char* op, int32_t count);
 
 /*
  * Device-side error flags of bounded waits in this library's kernels on
- * `device` (0 = none). clear != 0 resets them. Synchronizes `device`.
+ * `device` (0 = none, 1 = a copy's wait ran out, 2 = one of kvoff_attention_fp8;
+ * the result of that call means nothing). clear != 0 resets them. Synchronizes
+ * `device`.
  */
 KVOFF_API int kvoff_device_error(int32_t device, int32_t* flags, int32_t clear);
 
@@ -382,7 +384,7 @@ KVOFF_API int kvoff_store_kvcache_fp8(const void* key, int64_t key_stride_bytes,
  * leave their rows of out and lse as they were. max_seqlen_q is the longest
  * query length (it sizes the launch; the lengths themselves stay on the
  * device). Values in keys that a row does not see, NaN among them, do not
- * reach it.
+ * reach it. softmax_scale is positive and finite.
  *
  * head_dim is 64 or 128, page_size a multiple of 16, scale_block 16 * 2^n
  * tokens and a divisor of the page; q and the caches are 16-byte aligned.

@@ -196,7 +196,10 @@ extern "C" int kvoff_attention_fp8(
     return fail(KVOFF_EINVAL, "kvoff_attention_fp8: sizes exceed 32 bits");
   if (!(softmax_scale > 0.0f && softmax_scale < 3.4e38f))
     return fail(KVOFF_EINVAL, "kvoff_attention_fp8: softmax_scale must be positive and finite");
-  if (num_seqs == 0 || num_tokens == 0 || max_seqlen_q == 0) return ok();
+  if (num_seqs == 0 || num_tokens == 0) return ok();
+  if (max_seqlen_q < 1)
+    return fail(KVOFF_EINVAL, "kvoff_attention_fp8: max_seqlen_q %lld for %lld tokens",
+                (long long)max_seqlen_q, (long long)num_tokens);
   if (q == nullptr || out == nullptr || context_lens == nullptr ||
       (s.keys > 0 && (k_cache == nullptr || v_cache == nullptr || k_scale == nullptr ||
                       v_scale == nullptr || block_tables == nullptr)))

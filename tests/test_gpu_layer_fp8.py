@@ -617,6 +617,53 @@ def test_attention_results_do_not_depend_on_the_workspace(cuda):
     check_attention(batch, outs[0])
 
 
+def test_attention_refuses_a_workspace_that_is_too_small(cuda):
+    batch = build(generator(26), [(1, 3000)], 4, 1, 64, 16, 16, BF16)
+    q, kc, vc, ks, vs, tables, contexts, _ = batch
+    need = ops.attention_fp8_workspace(1, 1, tables.shape[1], 16, 4, 1, 64)
+    small = torch.empty(need - 1, dtype=torch.uint8, device=cuda)
+    with pytest.raises(kvoff.KvoffError, match=f"workspace of {need} bytes"):
+        ops.attention_fp8(q, kc, vc, ks, vs, tables, int32(contexts), workspace=small)
+    got = ops.attention_fp8(q, kc, vc, ks, vs, tables, int32(contexts),
+                            workspace=torch.empty(need, dtype=torch.uint8, device=cuda))
+    check_attention(batch, got)
+
+
+@pytest.mark.parametrize("n", [1, 20, 90])
+def test_attention_is_captured_on_its_first_call_and_repeats_itself(cuda, n):
+    """Two graphs of one call, replayed in turn and after other work: the same bits each time."""
+    lengths = [(n, 2500 + n), (n, n), (n, 1400 + n)]
+    batch = build(generator(27), lengths, 8, 2, 128, 64, 32, FP16)
+    q, kc, vc, ks, vs, tables, contexts, starts = batch
+    args = (q, kc, vc, ks, vs, tables, int32(contexts))
+    options = dict(cu_seqlens_q=int32(starts), max_seqlen_q=n)
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(ops.attention_fp8(*args, **options))
+        graphs.append(graph)
+    for graph in graphs + graphs:
+        graph.replay()
+    eager = ops.attention_fp8(*args, **options)
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], eager)
+    check_attention(batch, eager)
+
+
+def test_attention_many_sequences_of_every_length(cuda):
+    """More sequences than threads, most of them short, so that CTAs walk over many of them."""
+    g = generator(28)
+    contexts = torch.randint(0, 70, (700,), generator=g, device="cuda").tolist()
+    contexts[5], contexts[600] = 5000, 2600
+    batch = build(g, [(1, c) for c in contexts], 2, 1, 64, 16, 16, BF16)
+    check_attention(batch, call(batch, [(1, c) for c in contexts], decode=True))
+    lengths = [(min(c, 1 + i % 40), c) for i, c in enumerate(contexts[:120])]
+    batch = build(g, lengths, 2, 1, 64, 16, 16, BF16)
+    check_attention(batch, call(batch, lengths))
+
+
 def test_empty_calls_do_nothing(cuda):
     kc, ks = torch.zeros(2, 16, 1, 64, device=cuda).to(torch.float8_e4m3fn), torch.ones(2, 1, 1, device=cuda)
     none = torch.empty(0, 1, 64, dtype=BF16, device=cuda)

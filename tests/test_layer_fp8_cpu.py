@@ -70,6 +70,8 @@ def attention(**change):
     (dict(most=2), "one token"), (dict(q=None), "null"), (dict(contexts=None), "null"), (dict(tables=None), "null"),
     (dict(vs=None), "null"), (dict(q=ctypes.c_void_p(264)), "aligned"), (dict(vc=ctypes.c_void_p(264)), "aligned"),
     (dict(out=ctypes.c_void_p(258)), "aligned"), (dict(qs=1032), "aligned"),
+    (dict(starts=P, most=0), "max_seqlen_q"), (dict(scale=0.0), "softmax_scale"), (dict(scale=-1.0), "softmax_scale"),
+    (dict(scale=math.nan), "softmax_scale"), (dict(scale=math.inf), "softmax_scale"),
     (dict(starts=P, most=2 ** 30), "32 bits"), (dict(starts=P, n=2 ** 30), "32 bits"),
 ])
 def test_attention_refuses(change, message):
