@@ -440,11 +440,14 @@ def _raw_stream(index: int, stream) -> int:
     return _stream(torch.device("cuda", index), stream)
 
 
+_ONE_DEVICE = "the tensors must be CUDA tensors on one device"
+
+
 def _one_device(index: int, *tensors) -> None:
     """Refuse tensors that are not all on CUDA device `index` (-1: the first is not on any)."""
     for t in tensors:
         if index < 0 or t.get_device() != index:
-            raise ValueError("the tensors must be CUDA tensors on one device")
+            raise ValueError(_ONE_DEVICE)
 
 
 def _rows(x: torch.Tensor, what: str, size: int = 2) -> int:
@@ -557,7 +560,9 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: tor
             raise ValueError("the outputs must have the shapes of q and k")
     size = 4 if code == _lib.FP32 else 2
     index = q.get_device()
-    _one_device(index, k, positions, table)
+    if index < 0 or k.get_device() != index or positions.get_device() != index \
+            or table.get_device() != index:
+        raise ValueError(_ONE_DEVICE)
     q_stride, k_stride = _rows(q, "q", size), _rows(k, "k", size)
     if out is None:
         q_out_stride, k_out_stride = q_stride, k_stride
@@ -581,8 +586,10 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: tor
 
 
 def _fp8_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
-               v_scale: torch.Tensor) -> int:
-    """Check an e4m3 cache [pages, page, H, D] and its scales; tokens of a scale block."""
+               v_scale: torch.Tensor, index: int):
+    """Check an e4m3 cache [pages, page, H, D] and its scales, all on device `index` (-1: on any).
+
+    Returns the cache's shape and the tokens of a scale block."""
     shape, scales = k_cache.shape, k_scale.shape
     if len(shape) != 4 or v_cache.shape != shape:
         raise ValueError("k_cache and v_cache must be [pages, page, heads, head_dim], alike")
@@ -596,7 +603,10 @@ def _fp8_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tens
     if not (k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous()
             and v_scale.is_contiguous()):
         raise ValueError("caches and scales must be contiguous")
-    return shape[1] // scales[1]
+    if index >= 0 and not (k_cache.get_device() == index == v_cache.get_device()
+                           and k_scale.get_device() == index == v_scale.get_device()):
+        raise ValueError(_ONE_DEVICE)
+    return shape, shape[1] // scales[1]
 
 
 def store_kvcache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
@@ -620,15 +630,15 @@ def store_kvcache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Ten
     code = _DTYPES.get(dtype, _lib.FP32)
     if code == _lib.FP32 or value.dtype != dtype:
         raise ValueError("key and value must both be bf16 or fp16")
-    block = _fp8_cache(k_cache, v_cache, k_scale, v_scale)
-    pages, page, cache_heads, cache_dim = k_cache.shape
+    index = key.get_device()
+    (pages, page, cache_heads, cache_dim), block = _fp8_cache(k_cache, v_cache, k_scale, v_scale, index)
     if cache_heads != heads or cache_dim != dim:
         raise ValueError("cache slots must hold [H, D] rows")
     if slot_mapping.dtype != torch.int32 or slot_mapping.numel() != num_tokens \
             or not slot_mapping.is_contiguous():
         raise ValueError("slot_mapping must be contiguous int32, one slot per token")
-    index = key.get_device()
-    _one_device(index, value, k_cache, v_cache, k_scale, v_scale, slot_mapping)
+    if index < 0 or value.get_device() != index or slot_mapping.get_device() != index:
+        raise ValueError(_ONE_DEVICE)
     bad = 0
     if bad_slots is not None:
         if bad_slots.dtype != torch.int32 or bad_slots.numel() < 1:
@@ -667,15 +677,14 @@ def _workspace_bytes(index: int, sizes: tuple) -> int:
     return found
 
 
-def _empty_on(stream, index: int, shape, dtype: torch.dtype) -> torch.Tensor:
-    """An empty tensor whose memory belongs to `stream` (None: the current stream)."""
-    device = torch.device("cuda", index)
+def _empty_on(stream, q: torch.Tensor, shape, dtype: torch.dtype) -> torch.Tensor:
+    """An empty tensor on q's device whose memory belongs to `stream` (None: the current stream)."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return q.new_empty(shape, dtype=dtype)
     if not isinstance(stream, torch.cuda.Stream):
-        stream = torch.cuda.ExternalStream(_stream(device, stream), device=device)
+        stream = torch.cuda.ExternalStream(_stream(q.device, stream), device=q.device)
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return q.new_empty(shape, dtype=dtype)
 
 
 def attention_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -701,8 +710,8 @@ def attention_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     """
     q_shape = q.shape
     n, q_heads, dim = q_shape
-    block = _fp8_cache(k_cache, v_cache, k_scale, v_scale)
-    pages, page, kv_heads, cache_dim = k_cache.shape
+    index = q.get_device()
+    (pages, page, kv_heads, cache_dim), block = _fp8_cache(k_cache, v_cache, k_scale, v_scale, index)
     if cache_dim != dim:
         raise ValueError("q and the caches must have the same head_dim")
     dtype = q.dtype
@@ -718,8 +727,8 @@ def attention_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     if context_lens.dtype != torch.int32 or context_lens.shape != (seqs,) \
             or not context_lens.is_contiguous():
         raise ValueError("context_lens must be contiguous int32, one for each row of block_tables")
-    index = q.get_device()
-    _one_device(index, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens)
+    if index < 0 or block_tables.get_device() != index or context_lens.get_device() != index:
+        raise ValueError(_ONE_DEVICE)
     starts = 0
     if cu_seqlens_q is not None:
         if cu_seqlens_q.dtype != torch.int32 or cu_seqlens_q.shape != (seqs + 1,) \
@@ -730,7 +739,7 @@ def attention_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     elif n != seqs or max_seqlen_q != 1:
         raise ValueError("without cu_seqlens_q each sequence has one token")
     if out is None:
-        out = _empty_on(stream, index, q_shape, dtype)
+        out = _empty_on(stream, q, q_shape, dtype)
         out_stride = 2 * q_heads * dim
     else:
         if out.shape != q_shape or out.dtype != dtype:
@@ -747,7 +756,7 @@ def attention_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     if workspace is None:
         have = _workspace_bytes(index, (seqs, max_seqlen_q, width, page, q_heads, kv_heads, dim))
         if have:
-            workspace = _empty_on(stream, index, (have,), torch.uint8)
+            workspace = _empty_on(stream, q, (have,), torch.uint8)
             space = workspace.data_ptr()
     else:
         if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
