@@ -8,10 +8,9 @@
 // keeps about 160 KB of loads in flight on each SM, and spends as few
 // instructions a byte as it can. Measured: 4 sequences of 34816 keys, 32 / 8
 // heads of 128, in 59 us = 4.8 TB/s, 0.74 of a copy's rate; from 34816 to 69632
-// keys 5.5 TB/s and more are added, so about 10 us of it begin and end the call
-// (the walk over the lengths 1.8, first addresses 1.9, first tiles 1.5, the join
-// of the warps 1.3, the join kernel 2.3 us).
-//
+// keys it adds 5.95 TB/s, so about 11 us of it begin and end the call (the walk
+// over the lengths 1.8, first addresses 1.9, first tiles 1.5, the join of the
+// warps 1.3, the join kernel 2.3 us, the launches).
 //
 // * A warp works alone on 16-key tiles: its own ring of kStages tiles of K
 //   and V in shared memory, filled by cp.async, 4 KB a tile at D = 128. No
