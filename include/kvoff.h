@@ -323,7 +323,8 @@ enum kvoff_dtype { KVOFF_BF16 = 0, KVOFF_FP16 = 1, KVOFF_FP32 = 2 };
  * through. Row p of `table` [table_rows, rotary_dim] (fp32) holds position p's
  * cosines, then its sines. KVOFF_ROTARY_INVERSE applies the transposed map
  * (the gradient). Products are fp32, rounded once. q_out and k_out may be q
- * and k (in place) but must not overlap them otherwise. A token whose position
+ * and k (in place, at the same strides) but must not overlap them otherwise;
+ * tokens of an output must not overlap. A token whose position
  * is negative is skipped: nothing of it is written; one whose position is not
  * in the table is skipped and counted into *bad_positions when that is
  * non-null (device memory). Enqueues one kernel, allocates nothing.
@@ -381,7 +382,8 @@ KVOFF_API int kvoff_store_kvcache_fp8(const void* key, int64_t key_stride_bytes,
  * A page id that is negative or not below num_pages is not read: its keys
  * count as absent. A context longer than the table is cut to it; offsets of
  * cu_seqlens_q are cut to num_tokens. Tokens of q that belong to no sequence
- * leave their rows of out and lse as they were. max_seqlen_q is the longest
+ * leave their rows of out and lse as they were. out must not overlap q, nor its
+ * tokens one another. max_seqlen_q is the longest
  * query length (it sizes the launch; the lengths themselves stay on the
  * device). Values in keys that a row does not see, NaN among them, do not
  * reach it. softmax_scale is positive and finite.

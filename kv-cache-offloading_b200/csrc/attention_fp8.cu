@@ -210,6 +210,8 @@ extern "C" int kvoff_attention_fp8(
   if ((wide & 15u) != 0 || (pairs & 3u) != 0)
     return fail(KVOFF_EINVAL,
                 "kvoff_attention_fp8: q and the caches must be 16-byte aligned, out 4-byte");
+  if (num_tokens > 1 && out_stride_bytes < q_heads * head_dim * 2)
+    return fail(KVOFF_EINVAL, "kvoff_attention_fp8: rows of the output overlap");
   const attention::Choice c = attention::choose(s);
   const int64_t need = attention::workspace_of(c, head_dim);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need ||

@@ -107,10 +107,10 @@ struct Segment {
 
 // Deals the work of a launch over its CTAs. With stride kv_heads, CTA c has head
 // c % kv_heads, and the heads are dealt alike: CTAs that run side by side read
-// the same tokens' rows of all heads, which stand next to one another in memory
+// the same tokens' rows of all heads, which stand next to one another in memory.
 // With stride 1 the heads stand on the axis too. The key reads of all (sequence,
-// head, row tile) triples, and a fixed cost of each, stand on one axis, in that order; each CTA takes an
-// equal stretch of it, cut at key tiles. So a batch of unequal lengths, or one
+// head, row tile) triples, and a fixed cost of each, stand on one axis, in that
+// order; each CTA takes an equal stretch of it, cut at key tiles. So a batch of unequal lengths, or one
 // long sequence, keeps all SMs busy to the end, from lengths that only the
 // device knows. A triple that is cut is joined by join_kernel.
 //

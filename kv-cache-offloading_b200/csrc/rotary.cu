@@ -283,6 +283,8 @@ extern "C" int kvoff_rotary(const void* q, int64_t q_stride_bytes, void* q_out,
     return fail(KVOFF_EINVAL, "kvoff_rotary: positions are int32 or int64");
   if ((flags & ~(KVOFF_ROTARY_INTERLEAVED | KVOFF_ROTARY_INVERSE)) != 0)
     return fail(KVOFF_EINVAL, "kvoff_rotary: unknown flags %d", (int)flags);
+  if ((q_heads + kv_heads) * head_dim > 0x1FFFFFFFll)
+    return fail(KVOFF_EINVAL, "kvoff_rotary: a token's heads exceed 2 GB");
   if (num_tokens == 0) return ok();
   if (num_tokens > 0x7FFFFFFFll)
     return fail(KVOFF_EINVAL, "kvoff_rotary: %lld tokens exceed one launch",
@@ -305,6 +307,14 @@ extern "C" int kvoff_rotary(const void* q, int64_t q_stride_bytes, void* q_out,
   if (bits % narrow != 0 || (interleaved && head_dim % 2 != 0))
     return fail(KVOFF_EINVAL, "kvoff_rotary: rows must be aligned to %d bytes%s", narrow,
                 interleaved ? " and hold an even number of values" : "");
+  // Rows written on top of one another, or over rows that are still to be read.
+  if (num_tokens > 1 &&
+      ((q_heads > 0 && q_out_stride_bytes < q_heads * head_dim * elem) ||
+       (kv_heads > 0 && k_out_stride_bytes < kv_heads * head_dim * elem)))
+    return fail(KVOFF_EINVAL, "kvoff_rotary: rows of the output overlap");
+  if (num_tokens > 1 && ((q_heads > 0 && q == q_out && q_stride_bytes != q_out_stride_bytes) ||
+                         (kv_heads > 0 && k == k_out && k_stride_bytes != k_out_stride_bytes)))
+    return fail(KVOFF_EINVAL, "kvoff_rotary: in place the strides of input and output are equal");
   RotaryArgs a{};
   a.in[0] = static_cast<const uint8_t*>(q);
   a.in[1] = static_cast<const uint8_t*>(k);

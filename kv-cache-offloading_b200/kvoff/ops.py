@@ -453,10 +453,10 @@ def _one_device(index: int, *tensors) -> None:
 def _rows(x: torch.Tensor, what: str, size: int = 2) -> int:
     """Bytes from one token to the next of x [N, H, D] with dense heads of `size`-byte values."""
     token, head, value = x.stride()
-    _, heads, dim = x.shape
+    tokens, heads, dim = x.shape
     if (value != 1 and dim > 1) or (head != dim and heads > 1):
         raise ValueError(f"the heads of {what} must be dense")
-    return token * size
+    return (token if tokens > 1 else heads * dim) * size  # a stride of one row means nothing
 
 
 def rotary_table(positions: int, rotary_dim: int, *, base: float = 10000.0,

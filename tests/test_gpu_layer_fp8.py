@@ -674,3 +674,14 @@ def test_empty_calls_do_nothing(cuda):
     q = torch.ones(2, 1, 64, dtype=BF16, device=cuda)
     out = ops.attention_fp8(q, kc, kc, ks, ks, torch.empty(2, 0, dtype=torch.int32, device=cuda), int32([5, 0]))
     assert (out == 0).all()  # tables without pages: every context is cut to none
+
+
+def test_one_token_with_any_stride(cuda):
+    g = generator(31)
+    q = randn(g, 1, 4, 64).to(BF16)
+    odd = q.as_strided((1, 4, 64), (1, 64, 1))
+    table, positions = ops.rotary_table(100, 64, device=cuda), torch.tensor([7], device=cuda)
+    out = torch.empty_like(q), torch.empty_like(q)
+    ops.rotary(odd, odd, positions, table, out=out)
+    check_rotary(q, out[0], positions, table, False, False)
+    check_rotary(q, out[1], positions, table, False, False)

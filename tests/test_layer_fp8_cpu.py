@@ -27,7 +27,8 @@ def rotary(**change):
     (dict(rot=0), "even"), (dict(dtype=7), "dtype"), (dict(pb=2), "int64"), (dict(flags=8), "flags"),
     (dict(q=None), "null"), (dict(ko=None), "null"), (dict(pos=None), "null"), (dict(table=None), "null"),
     (dict(q=ctypes.c_void_p(257)), "aligned"), (dict(flags=1, dim=65), "even number"),
-    (dict(flags=1, qs=514), "aligned"), (dict(n=2 ** 31), "exceed"),
+    (dict(flags=1, qs=514), "aligned"), (dict(n=2 ** 31), "exceed"), (dict(hq=65000, dim=65000), "exceed"),
+    (dict(qos=256), "overlap"), (dict(kos=128), "overlap"), (dict(qs=1024), "in place"), (dict(kos=1024), "in place"),
 ])
 def test_rotary_refuses(change, message):
     assert rotary(**change) == _lib.KVOFF_EINVAL
@@ -72,11 +73,17 @@ def attention(**change):
     (dict(out=ctypes.c_void_p(258)), "aligned"), (dict(qs=1032), "aligned"),
     (dict(starts=P, most=0), "max_seqlen_q"), (dict(scale=0.0), "softmax_scale"), (dict(scale=-1.0), "softmax_scale"),
     (dict(scale=math.nan), "softmax_scale"), (dict(scale=math.inf), "softmax_scale"),
-    (dict(starts=P, most=2 ** 30), "32 bits"), (dict(starts=P, n=2 ** 30), "32 bits"),
+    (dict(starts=P, most=2 ** 30), "32 bits"), (dict(starts=P, n=2 ** 30), "32 bits"), (dict(os=256), "overlap"),
 ])
 def test_attention_refuses(change, message):
     assert attention(**change) == _lib.KVOFF_EINVAL
     assert message in _lib.last_error()
+
+
+def test_the_stride_of_one_row_means_nothing():
+    x = torch.zeros(4, 64, 1, dtype=torch.bfloat16).permute(2, 0, 1)
+    assert x.stride(0) == 1 and ops._rows(x, "x") == 4 * 64 * 2
+    assert ops._rows(torch.zeros(3, 6, 64)[:, :4], "x", 4) == 6 * 64 * 4
 
 
 def test_empty_calls_are_accepted_without_a_device():
