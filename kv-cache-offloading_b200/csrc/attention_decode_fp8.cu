@@ -28,11 +28,16 @@
 //   brought together byte by byte (prmt) and converted like K; P goes from the
 //   accumulator layout to the operand's by movmatrix. The scale of V is one
 //   number for the tile (a scale block is 16 tokens or more) and is put into
-//   P, as a fraction of the largest scale met so far, times 2^8, so that f16
-//   holds weights down to 2^-22 of the largest at full precision.
-// * The running maximum is raised only when a score passes it by more than
-//   2^6 (one vote a tile); until then P is at most 2^14 in f16. Rescaling is
-//   rare then, and the reductions over keys stay out of the loop.
+//   P = 2^(x - m) scale / 2^t, where 2^(m + t + 8) follows the largest 2^x scale
+//   that the row itself has met: f16 holds terms down to 2^-22 of the row's
+//   largest one at full precision, whatever scales other rows' keys have, or
+//   keys of no weight. Keys whose V is all zero do not count there: beside a
+//   large value, seen or not, a scale block holds nothing else. The sum of
+//   2^(x - m) does not depend on t.
+// * m and t are raised only when a score, or a score with its scale, passes
+//   them by more than 2^6 (one vote a tile, on the lower of the two limits); until
+//   then P is at most 2^14 in f16. Rescaling is rare then, and the reductions over
+//   keys stay out of the loop.
 //
 // Masked scores are -inf before anything depends on them. Rows of K and V
 // behind the context are not read (cp.async fills zeros), since 0 * NaN would
@@ -49,7 +54,8 @@ constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kTile = 16;           // keys of a warp's tile
 constexpr float kRaise = 6.0f;      // log2 of how far P may pass 1
-constexpr float kWeight = 256.0f;   // of P in f16
+constexpr float kWeightLog2 = 8.0f; // of the largest P in f16
+constexpr float kLeastUnit = -126.0f;  // of t
 constexpr uint32_t kNegInf = 0xFF800000u;
 static_assert(kKeyTile == kWarps * kTile, "one tile a warp and key tile");
 
@@ -180,6 +186,18 @@ struct VTile {
       }
     }
   }
+  // The first of the tile's keys that this thread has a value of V for that is not zero, or kTile.
+  __device__ __forceinline__ uint32_t first_nonzero(int t) const {
+    uint32_t first = kTile;
+#pragma unroll
+    for (int i = 3; i >= 0; --i) {
+      uint32_t any = 0;
+#pragma unroll
+      for (int k = 0; k < kWords; ++k) any |= w[i][k];
+      if ((any & 0x7F7F7F7Fu) != 0) first = 2 * t + (i & 1) + (i >> 1) * 8;
+    }
+    return first;
+  }
   // Fragment of M tile i (values d0 + 2i in rows g, d0 + 2i + 1 in rows g + 8).
   __device__ __forceinline__ void fragment(int i, uint32_t (&a)[4]) const {
     const uint32_t pick = (i & 1) ? 0x7362 : 0x5140;  // bytes 2, 3 or 0, 1 of both keys
@@ -190,6 +208,9 @@ struct VTile {
   }
 };
 
+// 2^x. Past 2^126 it meets scores whose 2^(x - m) is 0 in fp32 only.
+__device__ __forceinline__ float weight_of(float x) { return exp2_fast(x > 126.0f ? 126.0f : x); }
+
 // One warp's state over a segment.
 template <int D, int NT>
 struct Rows {
@@ -198,8 +219,8 @@ struct Rows {
   float factor[NT][2];        // log2 units of a raw score, columns 2t and 2t+1
   int limit[NT][2];           // keys that the column's row sees
   float o[kSteps][NT][4];
-  float m[NT][2], l[NT][2];
-  float ref, inverse;  // largest V scale met, and its reciprocal times kWeight
+  float m[NT][2], l[NT][2];   // l: sum of 2^(x - m)
+  float unit[NT][2];          // t: o is the sum of 2^(x - m - t) v
 };
 
 template <int D, int NT>
@@ -262,9 +283,11 @@ __device__ __forceinline__ void load_rows(const Args& a, const Sequence& seq, co
       const int column = 2 * t + i;
       r.factor[j][i] = __shfl_sync(0xFFFFFFFFu, down, column * 4);
       const int at = seg.tile * a.rows + 8 * j + column;
-      r.limit[j][i] = at < total ? max(0, seq.context - seq.q_len + at / a.group + 1) : 0;
+      // A column without a row has q = 0 and sees all keys: it asks for nothing.
+      r.limit[j][i] = at < total ? max(0, seq.context - seq.q_len + at / a.group + 1) : 0x7FFFFFFF;
       r.m[j][i] = __uint_as_float(kNegInf);
       r.l[j][i] = 0.0f;
+      r.unit[j][i] = kLeastUnit;
     }
   }
 #pragma unroll
@@ -273,8 +296,6 @@ __device__ __forceinline__ void load_rows(const Args& a, const Sequence& seq, co
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int k = 0; k < 4; ++k) r.o[i][j][k] = 0.0f;
-  r.ref = 0.0f;
-  r.inverse = 0.0f;
 }
 
 // O += V^T P^T of a tile where some of V is NaN and some rows do not see all
@@ -462,21 +483,27 @@ __global__ void __launch_bounds__(kThreads, 1) attention_decode_fp8_kernel(const
 
           // Scores in log2 units; x[j][k] is key g + 8 (k / 2), column 2t + k % 2.
           const bool masked = (tile + 1) * kTile > fewest;
-          bool raise = scales.y > r.ref;
+          const float v_log2 = scale_log2_of(scales.y);
+          float weight[NT][2];  // scale / 2^t
+          bool raise = false;
 #pragma unroll
-          for (int j = 0; j < NT; ++j)
+          for (int j = 0; j < NT; ++j) {
+            float most[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              most[k] = r.m[j][k] + kRaise + fminf(0.0f, r.unit[j][k] + kWeightLog2 - v_log2);
+              weight[j][k] = weight_of(v_log2 - r.unit[j][k]);
+            }
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               x[j][k] = (x[j][k] + odd[j][k]) * (scales.x * r.factor[j][k & 1]);
               if (masked && tile * kTile + g + 8 * (k >> 1) >= r.limit[j][k & 1])
                 x[j][k] = __uint_as_float(kNegInf);
-              raise = raise || x[j][k] > r.m[j][k & 1] + kRaise;
+              raise = raise || x[j][k] > most[k & 1];
             }
+          }
           if (__any_sync(0xFFFFFFFFu, raise)) {
-            const float ref = fmaxf(r.ref, scales.y);
-            const float ratio = ref > 0.0f ? r.ref / ref : 1.0f;
-            r.ref = ref;
-            r.inverse = ref > 0.0f ? kWeight / fmaxf(ref, 1e-36f) : 0.0f;
+            const int first = (int)__reduce_min_sync(0xFFFFFFFFu, v.first_nonzero(t));
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
               float keep[2];
@@ -486,11 +513,17 @@ __global__ void __launch_bounds__(kThreads, 1) attention_decode_fp8_kernel(const
                 most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 4));
                 most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 8));
                 most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 16));
-                most = fmaxf(most, r.m[j][k]);
-                keep[k] = most == r.m[j][k] ? 1.0f : exp2_fast(r.m[j][k] - most);
+                const float m = r.m[j][k], unit = r.unit[j][k];
+                const float column_log2 = first < min(r.limit[j][k] - tile * kTile, kTile) ? v_log2 : kZeroLog2;
+                const float term = most + column_log2 - kWeightLog2;
+                most = fmaxf(most, m);
+                // (-inf) - (-inf) and inf - inf, of a row that has seen nothing or infinities, are none.
+                const float next = fmaxf(fmaxf(m + unit, term) - most, kLeastUnit);
+                keep[k] = most == m && next == unit ? 1.0f : exp2_fast((m + unit) - (most + next));
+                if (most != m) r.l[j][k] *= exp2_fast(m - most);
                 r.m[j][k] = most;
-                r.l[j][k] *= keep[k];
-                keep[k] *= ratio;
+                r.unit[j][k] = next;
+                weight[j][k] = weight_of(column_log2 - next);
               }
 #pragma unroll
               for (int n = 0; n < kSteps; ++n)
@@ -498,7 +531,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_decode_fp8_kernel(const
                 for (int k = 0; k < 4; ++k) r.o[n][j][k] *= keep[k & 1];
             }
           }
-          const float weight = scales.y * r.inverse;
           uint32_t p[NT][2], seen[NT][2];
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
@@ -510,8 +542,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_decode_fp8_kernel(const
               e[k] = exp2_fast(x[j][k] - (m == __uint_as_float(kNegInf) ? 0.0f : m));
               r.l[j][k & 1] += e[k];
             }
-            p[j][0] = transpose8x8(pack_half(e[0] * weight, e[1] * weight));
-            p[j][1] = transpose8x8(pack_half(e[2] * weight, e[3] * weight));
+            p[j][0] = transpose8x8(pack_half(e[0] * weight[j][0], e[1] * weight[j][1]));
+            p[j][1] = transpose8x8(pack_half(e[2] * weight[j][0], e[3] * weight[j][1]));
           }
           // Only a tile that the rows see to different lengths can hold NaN that a
           // row must not meet: behind the context there are zeros.
@@ -589,8 +621,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_decode_fp8_kernel(const
 #pragma unroll
           for (int w = 1; w < kWarps; ++w) most = fmaxf(most, warp_m[w][column]);
           const float m = r.m[j][k];
-          const float keep =
-              (m == __uint_as_float(kNegInf) ? 0.0f : exp2_fast(m - most)) * (r.ref / kWeight);
+          const float keep = m == __uint_as_float(kNegInf) ? 0.0f : exp2_fast(m - most + r.unit[j][k]);
 #pragma unroll
           for (int n = 0; n < kSteps; ++n)
             *reinterpret_cast<float2*>(sums + column * kPitch + D / 8 * g + 2 * n) =

@@ -297,6 +297,15 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// log2 of a scale of V. One that is zero is far below all others: its keys
+// count in the sum of weights only. So do keys whose V is all zero.
+constexpr float kZeroLog2 = -200.0f;
+__device__ __forceinline__ float scale_log2_of(float scale) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(scale));
+  return scale > 0.0f ? fmaxf(y, kZeroLog2) : scale == scale ? kZeroLog2 : scale;
+}
+
 // Writes two adjacent output values of a row.
 __device__ __forceinline__ void write_pair(const Args& a, int token, int q_head, int dim, int d,
                                            float x, float y) {
