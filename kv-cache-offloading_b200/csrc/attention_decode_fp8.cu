@@ -32,7 +32,7 @@
 //   that the row itself has met: f16 holds terms down to 2^-22 of the row's
 //   largest one at full precision, whatever scales other rows' keys have, or
 //   keys of no weight. Keys whose V is all zero do not count there: beside a
-//   large value, seen or not, a scale block holds nothing else. The sum of
+//   large value, seen or not, a scale block holds little else. The sum of
 //   2^(x - m) does not depend on t.
 // * m and t are raised only when a score, or a score with its scale, passes
 //   them by more than 2^6 (one vote a tile, on the lower of the two limits); until
@@ -186,17 +186,22 @@ struct VTile {
       }
     }
   }
-  // The first of the tile's keys that this thread has a value of V for that is not zero, or kTile.
-  __device__ __forceinline__ uint32_t first_nonzero(int t) const {
-    uint32_t first = kTile;
+  // The tile's keys with a value that is not zero, one bit each. All lanes of the warp call it.
+  __device__ __forceinline__ uint32_t filled() const {
+    uint32_t keys = 0;
 #pragma unroll
-    for (int i = 3; i >= 0; --i) {
+    for (int i = 0; i < 4; ++i) {
       uint32_t any = 0;
 #pragma unroll
       for (int k = 0; k < kWords; ++k) any |= w[i][k];
-      if ((any & 0x7F7F7F7Fu) != 0) first = 2 * t + (i & 1) + (i >> 1) * 8;
+      uint32_t lanes = __ballot_sync(0xFFFFFFFFu, (any & 0x7F7F7F7Fu) != 0);
+      lanes |= lanes >> 16;
+      lanes |= lanes >> 8;
+      lanes |= lanes >> 4;  // bit t: key 2t + (i & 1) + 8 (i >> 1)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) keys |= (lanes >> t & 1) << (2 * t + (i & 1) + (i >> 1) * 8);
     }
-    return first;
+    return keys;
   }
   // Fragment of M tile i (values d0 + 2i in rows g, d0 + 2i + 1 in rows g + 8).
   __device__ __forceinline__ void fragment(int i, uint32_t (&a)[4]) const {
@@ -207,6 +212,13 @@ struct VTile {
     a[2] = widen_low(high), a[3] = widen_high(high);
   }
 };
+
+// The largest of a column's values, over the lanes that hold its keys.
+__device__ __forceinline__ float column_most(float x) {
+  x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 4));
+  x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 8));
+  return fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 16));
+}
 
 // 2^x. Past 2^126 it meets scores whose 2^(x - m) is 0 in fp32 only.
 __device__ __forceinline__ float weight_of(float x) { return exp2_fast(x > 126.0f ? 126.0f : x); }
@@ -283,8 +295,7 @@ __device__ __forceinline__ void load_rows(const Args& a, const Sequence& seq, co
       const int column = 2 * t + i;
       r.factor[j][i] = __shfl_sync(0xFFFFFFFFu, down, column * 4);
       const int at = seg.tile * a.rows + 8 * j + column;
-      // A column without a row has q = 0 and sees all keys: it asks for nothing.
-      r.limit[j][i] = at < total ? max(0, seq.context - seq.q_len + at / a.group + 1) : 0x7FFFFFFF;
+      r.limit[j][i] = at < total ? max(0, seq.context - seq.q_len + at / a.group + 1) : 0;
       r.m[j][i] = __uint_as_float(kNegInf);
       r.l[j][i] = 0.0f;
       r.unit[j][i] = kLeastUnit;
@@ -491,7 +502,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_decode_fp8_kernel(const
             float most[2];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-              most[k] = r.m[j][k] + kRaise + fminf(0.0f, r.unit[j][k] + kWeightLog2 - v_log2);
+              most[k] = r.m[j][k] + fminf(kRaise, r.unit[j][k] + (kWeightLog2 + kRaise) - v_log2);
               weight[j][k] = weight_of(v_log2 - r.unit[j][k]);
             }
 #pragma unroll
@@ -503,27 +514,37 @@ __global__ void __launch_bounds__(kThreads, 1) attention_decode_fp8_kernel(const
             }
           }
           if (__any_sync(0xFFFFFFFFu, raise)) {
-            const int first = (int)__reduce_min_sync(0xFFFFFFFFu, v.first_nonzero(t));
+            const uint32_t filled = v.filled();
+            const bool some_empty = filled != 0xFFFFu;
+            const bool empty[2] = {(filled >> g & 1) == 0, (filled >> (g + 8) & 1) == 0};
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
               float keep[2];
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
-                float most = fmaxf(x[j][k], x[j][k + 2]);
-                most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 4));
-                most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 8));
-                most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 16));
+                float most = column_most(fmaxf(x[j][k], x[j][k + 2])), most_filled = most;
                 const float m = r.m[j][k], unit = r.unit[j][k];
-                const float column_log2 = first < min(r.limit[j][k] - tile * kTile, kTile) ? v_log2 : kZeroLog2;
-                const float term = most + column_log2 - kWeightLog2;
                 most = fmaxf(most, m);
+                if (most != m) r.l[j][k] *= exp2_fast(m - most);
+                if (some_empty) {
+                  // Keys of zeros count in l and are taken out: they add nothing to o,
+                  // and P with their scale may not fit f16.
+                  const float base = most == __uint_as_float(kNegInf) ? 0.0f : most;
+#pragma unroll
+                  for (int n = 0; n < 2; ++n)
+                    if (empty[n]) {
+                      r.l[j][k] += exp2_fast(x[j][k + 2 * n] - base);
+                      x[j][k + 2 * n] = __uint_as_float(kNegInf);
+                    }
+                  most_filled = column_most(fmaxf(x[j][k], x[j][k + 2]));
+                }
+                const float term = most_filled + v_log2 - kWeightLog2;
                 // (-inf) - (-inf) and inf - inf, of a row that has seen nothing or infinities, are none.
                 const float next = fmaxf(fmaxf(m + unit, term) - most, kLeastUnit);
                 keep[k] = most == m && next == unit ? 1.0f : exp2_fast((m + unit) - (most + next));
-                if (most != m) r.l[j][k] *= exp2_fast(m - most);
                 r.m[j][k] = most;
                 r.unit[j][k] = next;
-                weight[j][k] = weight_of(column_log2 - next);
+                weight[j][k] = weight_of(v_log2 - next);
               }
 #pragma unroll
               for (int n = 0; n < kSteps; ++n)

@@ -129,24 +129,26 @@ def test_decode_kernel_later_keys_of_large_values(cuda, value, inside, lengths, 
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP16])
-@pytest.mark.parametrize("first", [False, True])
+@pytest.mark.parametrize("first,low", [(False, None), (True, None), (False, 4), (False, 1), (True, 4)])
 @pytest.mark.parametrize("lengths,q_heads,kv_heads,dim,page,block", FEW + [([(1, 130), (1, 3000)], 8, 1, 128, 64, 32)])
-def test_decode_kernel_large_values_of_little_weight(cuda, dtype, first, lengths, q_heads, kv_heads, dim, page, block):
-    check_little_weight(2, dtype, first, lengths, q_heads, kv_heads, dim, page, block)
+def test_decode_kernel_large_values_of_little_weight(cuda, dtype, first, low, lengths, q_heads, kv_heads, dim, page, block):
+    check_little_weight(2, dtype, first, low, lengths, q_heads, kv_heads, dim, page, block)
 
 
-def check_little_weight(seed, dtype, first, lengths, q_heads, kv_heads, dim, page, block):
-    """The first scale block has large V and scores so low that it counts for less than the rest does; with `first`
-    its scores are not as low and it decides the result."""
+def check_little_weight(seed, dtype, first, low, lengths, q_heads, kv_heads, dim, page, block):
+    """The first `low` keys (None: a scale block) have large V and scores so low that they count for less than the
+    rest does; with `first` their scores are not as low and they decide the result. The other keys of their block,
+    whose payload is zero, have weight."""
+    low = low or block
     batch = Batch(seed, lengths, q_heads, kv_heads, dim, page, block, dtype)
     batch.q[..., 0] = 4.0
     for (n, c), (k, v) in zip(batch.lengths, batch.rows):
         k[..., 0] = 0.0
-        k[:block, :, 0] = -8.0 if first else -64.0  # 4 * 64 / sqrt(dim) is 22 or 32 below the others' scores
-        v[:block] *= 2.0 ** ((60 if first else 30 if dim == 128 else 44) if dtype == BF16 else 12)
+        k[:low, :, 0] = -8.0 if first else -64.0  # 4 * 64 / sqrt(dim) is 22 or 32 below the others' scores
+        v[:low] *= 2.0 ** ((60 if first else 30 if dim == 128 else 44) if dtype == BF16 else 12)
         if c > 600:  # another CTA's part
-            k[416:416 + block, :, 0] = -48.0
-            v[416:416 + block] *= 2.0 ** 20 if dtype == BF16 else 1.0
+            k[416:416 + low, :, 0] = -48.0
+            v[416:416 + low] *= 2.0 ** 20 if dtype == BF16 else 1.0
     batch.check()
 
 
