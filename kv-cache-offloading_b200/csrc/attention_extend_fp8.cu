@@ -20,11 +20,14 @@
 // power of two to an amax of 2^14..2^15, where every bf16 value down to 2^-31
 // of the row's largest is exact. The scores S = Q K^T are fp32 in tensor
 // memory; a scale block is 16 tokens or more, so the scale of K enters once
-// per 16 scores. P = exp2(x - m) takes the scale of V with it, as a fraction
-// of the largest met so far (bias in the exponent), times 2^8, and goes back
-// to tensor memory as the f16 operand of O += P V, in the place of its scores.
-// The sum of p is taken before that, per 16 keys, and divided by the same
-// factor. The maximum is raised only when a score passes it by 2^6, so the
+// per 16 scores. P = 2^(x - m) takes the scale of V with it, as a fraction of
+// 2^(n - m) (bias in the exponent), times 2^8, and goes back to tensor memory as
+// the f16 operand of O += P V, in the place of its scores. n follows the largest
+// x + log2(scale) that the row itself has met, so its terms keep their bits
+// whatever scales other rows' keys have, or keys of no weight. Keys whose V is all
+// zero do not count there: beside a large value, seen or not, a scale block holds
+// little else. The sum of p is taken before that, per 16 keys, and divided by the
+// same factor. m and n are raised only when they are passed by 6, so the
 // accumulator is rescaled a few times in a row tile, not once in each key tile.
 //
 // Scores are made 64 keys at a time, in two sets of columns that take turns: the
@@ -61,7 +64,7 @@ constexpr int kTileRing = 4;       // pages and scales of a tile, ahead of K and
 constexpr int kWorkRing = 2;       // segments handed out ahead
 constexpr float kRaise = 6.0f;     // log2 of how far P may pass 1
 constexpr float kWeightLog2 = 8.0f;
-constexpr float kLeastLog2 = -42.0f;  // of a V scale against the largest: P rounds to 0 in f16
+constexpr float kLeastLog2 = -42.0f;  // of a V scale against 2^(n - m): P rounds to 0 in f16
 constexpr uint32_t kNegInf = 0xFF800000u;
 constexpr uint32_t kWaitNs = 1000, kMostWaits = 1u << 20;  // a second in all
 constexpr uint32_t kTmemColumns = 512;
@@ -79,18 +82,13 @@ struct Layout {
   static constexpr int kBytes = kNan + kStages * kNanBytes + 1024;  // 1024: alignment
 };
 
-// A key tile's 16-key groups: where they are and their scales. The scale of V
-// is a fraction of the largest one that the segment has met, times 2^8: it is
-// added to the exponent of P, and its inverse takes it out of the sum of p again.
+// A key tile's 16-key groups: where they are and their scales.
 struct Tile {
   int64_t place[8];  // byte of the cache, at this head; negative: no page
   float k[8];
-  float shift[8];    // log2
-  float inverse[8];
-  float largest;     // log2 of the largest scale of V so far
+  float v[8];        // log2
   uint32_t absent;   // bit g: group g has no page
   int32_t run;       // all 128 keys are read and follow one another from place[0]
-  int32_t pad;
 };
 
 // One segment, as the roles need it.
@@ -119,6 +117,7 @@ struct Shared {
   uint64_t tile_full[kTileRing];
   uint64_t drained[2];
   Tile tiles[kTileRing];
+  uint32_t filled[kStages][8];  // of V's 16-key groups: four bits a byte, 0: the key is all zero
   uint32_t nan[kStages];  // n + 1: V of tile n, in this stage, holds NaN that some row must not meet
   uint32_t tmem;
   uint64_t work_full[kWorkRing], work_empty[kWorkRing];
@@ -438,6 +437,31 @@ struct Convert {
     }
   }
 
+  // Notes the keys with a value that is not zero. A warp has 4 keys of each group, or
+  // 8 of every other one (D = 64), and all their chunks.
+  __device__ __forceinline__ void note_filled(int stage, const uint4 (&raw)[kPasses]) const {
+    const int lane = t % 32, warp = t / 32;
+    uint32_t mine = 0;  // of pass `lane`: the threads whose chunk is not zero
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const uint32_t any = (raw[i].x | raw[i].y | raw[i].z | raw[i].w) & 0x7F7F7F7Fu;
+      const uint32_t mask = __ballot_sync(0xFFFFFFFFu, any != 0);
+      if (lane == i) mine = mask;
+    }
+    if (lane >= kPasses) return;
+    if (D == 128) {
+      const uint32_t keys = ((mine & 0x0F0Fu) != 0 ? 1 : 0) | ((mine & 0xF0F0u) != 0 ? 2 : 0) |
+                            ((mine & 0x0F0F0000u) != 0 ? 4 : 0) | ((mine & 0xF0F00000u) != 0 ? 8 : 0);
+      reinterpret_cast<uint8_t*>(&sh->filled[stage][lane])[warp] = (uint8_t)keys;
+    } else {
+      uint32_t keys = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if ((mine >> 4 * i & 0xFu) != 0) keys |= 1u << (i + i / 4 * 4);
+      reinterpret_cast<uint16_t*>(&sh->filled[stage][2 * lane + warp / 2])[warp % 2] = (uint16_t)keys;
+    }
+  }
+
   // Takes NaN out of V and notes them, one bit each, per key and chunk.
   __device__ __forceinline__ void take_nan(int stage, uint32_t count, uint4 (&raw)[kPasses], uint8_t* masks) const {
 #pragma unroll
@@ -482,6 +506,7 @@ __device__ __forceinline__ void convert_role(const Args& a, Shared* sh, uint8_t*
       if (tile >= begin) {
         const int stage = count % kStages;
         bar_wait(&empty[stage], (count / kStages & 1) ^ 1, patience);
+        if (is_v) c.note_filled(stage, raw);
         if (is_v && work->mixed(tile)) c.take_nan(stage, count, raw, smem + L::kNan + stage * L::kNanBytes);
         c.put(operand + stage * L::kOperand, raw);
         async_fence();
@@ -522,7 +547,6 @@ __device__ __forceinline__ void tile_role(const Args& a, Shared* sh) {
       return lane < 8 && tile < end && key < keys ? __ldg(table + page_index(a, key)) : -1;
     };
     int page_next = page_of(begin);
-    float largest = -200.0f;
 #pragma unroll 1
     for (int tile = begin; tile < end; ++tile, ++count) {
       const int page = page_next < a.num_pages ? page_next : -1;
@@ -537,28 +561,17 @@ __device__ __forceinline__ void tile_role(const Args& a, Shared* sh) {
         v_scale = __ldg(a.scale[1] + at);
       }
       const uint32_t absent = __ballot_sync(0xFFFFFFFFu, page < 0) & 0xFFu;
-      float log2;
-      asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(log2) : "f"(v_scale));
-      log2 = v_scale > 0.0f ? fmaxf(log2, -200.0f) : v_scale == v_scale ? -200.0f : v_scale;
-      float most = lane < 8 ? log2 : -200.0f;
-#pragma unroll
-      for (int d = 4; d > 0; d /= 2) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
-      largest = fmaxf(largest, __shfl_sync(0xFFFFFFFFu, most, 0));
       if (count >= 2) {  // each phase in turn: a wait tells the last two apart only
         const uint32_t scores = count - 2;
         bar_wait(&sh->k_empty[scores % kStages], scores / kStages & 1, patience);
       }
       Tile& t = sh->tiles[count % kTileRing];
       if (lane < 8) {
-        const float relative = log2 - largest;
-        const float shift = (relative < kLeastLog2 ? kLeastLog2 : relative) + kWeightLog2;
         t.place[lane] = place;
         t.k[lane] = k_scale;
-        t.shift[lane] = shift;
-        t.inverse[lane] = exp2_fast(-shift);
+        t.v[lane] = scale_log2_of(v_scale);
       }
       if (lane == 0) {
-        t.largest = largest;
         t.absent = absent;
         t.run = long_pages && keys - tile * kKeyTile >= kKeyTile && absent == 0;
       }
@@ -675,27 +688,48 @@ __device__ __forceinline__ float factor_of(const Tile& scales, int b, float fact
   return fmaxf(scales.k[b] * factor, 1e-37f);
 }
 
-// The largest of the 32 scores of chunk c, in log2 units.
-__device__ __forceinline__ float top_of(const float (&s)[32], const Tile& scales, int c, float factor) {
+// The largest scores of the two groups of chunk c, in log2 units.
+__device__ __forceinline__ void top_of(const float (&s)[32], const Tile& scales, int c, float factor, float* most) {
   float top[4] = {s[0], s[1], s[16], s[17]};
 #pragma unroll
   for (int i = 2; i < 16; i += 2) {
     top[0] = fmaxf(top[0], s[i]), top[1] = fmaxf(top[1], s[i + 1]);
     top[2] = fmaxf(top[2], s[16 + i]), top[3] = fmaxf(top[3], s[17 + i]);
   }
-  return fmaxf(fmaxf(top[0], top[1]) * factor_of(scales, 2 * c, factor),
-               fmaxf(top[2], top[3]) * factor_of(scales, 2 * c + 1, factor));
+  most[0] = fmaxf(top[0], top[1]) * factor_of(scales, 2 * c, factor);
+  most[1] = fmaxf(top[2], top[3]) * factor_of(scales, 2 * c + 1, factor);
 }
 
+__device__ __forceinline__ float largest_of(const float (&x)[4]) { return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])); }
+
+// The largest of the four groups' scores with their V scales.
+__device__ __forceinline__ float term_of(const float (&x)[4], const float (&v)[4]) {
+  return fmaxf(fmaxf(x[0] + v[0], x[1] + v[1]), fmaxf(x[2] + v[2], x[3] + v[3]));
+}
+
+// The exponents of P: 2^(x + max(v + scaled, least)). `scaled` is 8 - n and `least`
+// kLeastLog2 + 8 - m, with m = n = 0 for a row that has seen nothing.
+struct Bias {
+  float m = 0.0f, scaled = kWeightLog2, least = kLeastLog2 + kWeightLog2;
+
+  __device__ __forceinline__ void set(float m_, float n) {
+    const bool none = m_ == __uint_as_float(kNegInf);
+    m = none ? 0.0f : m_;
+    scaled = kWeightLog2 - (none ? 0.0f : n);
+    least = kLeastLog2 + kWeightLog2 - m;
+  }
+};
+
 // P of the 32 scores of chunk c; its sums go into l. P takes the columns of
-// scores that have been read: 16 for these 32.
-__device__ __forceinline__ void weigh(const float (&s)[32], const Tile& scales, int c, float factor, float shift,
-                                      uint32_t scores_at, float& l) {
+// scores that have been read: 16 for these 32. `v`: V scales of the two groups.
+__device__ __forceinline__ void weigh(const float (&s)[32], const Tile& scales, int c, float factor, const Bias& from,
+                                      const float* v, uint32_t scores_at, float& l) {
   uint32_t p[16];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int b = 2 * c + k;
-    const float f = factor_of(scales, b, factor), bias = scales.shift[b] - shift;
+    const float f = factor_of(scales, b, factor), scaled = v[k] + from.scaled;
+    const float bias = scaled < from.least ? from.least : scaled;
     float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0;
 #pragma unroll
     for (int i = 0; i < 16; i += 4) {
@@ -707,9 +741,32 @@ __device__ __forceinline__ void weigh(const float (&s)[32], const Tile& scales, 
       p[8 * k + i / 2 + 1] = pack_half(y.x, y.y);
     }
     sum0 = add_pair(sum0, sum1);
-    l = fmaf(sum0.x + sum0.y, scales.inverse[b], l);
+    l = fmaf(sum0.x + sum0.y, exp2_fast(-(bias + from.m)), l);
   }
   tensor_store16(scores_at + 16 * (c % 2), p);
+}
+
+// Which of the 32 keys of chunk c are not all zero in V.
+__device__ __forceinline__ uint32_t filled_of(const uint32_t* filled, int c) {
+  uint32_t keys = 0;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const uint32_t w = filled[2 * c + k];
+    keys |= (w & 0xFu | w >> 4 & 0xF0u | w >> 8 & 0xF00u | w >> 12 & 0xF000u) << 16 * k;
+  }
+  return keys;
+}
+
+// Adds the weights of chunk c's other keys to l, and takes the keys out: they add
+// nothing to O, and P with their scale may not fit f16.
+__device__ __forceinline__ void set_aside(float (&s)[32], const Tile& scales, int c, float factor, float m,
+                                          uint32_t filled, float& l) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if ((filled >> i & 1) == 0) {
+      l += exp2_fast(fmaf(s[i], factor_of(scales, 2 * c + i / 16, factor), -m));
+      s[i] = __uint_as_float(kNegInf);
+    }
 }
 
 template <int D>
@@ -769,7 +826,8 @@ __device__ __forceinline__ void softmax_role(const Args& a, Shared* sh, uint8_t*
       tensor_fence_before();
       warp_arrive(&sh->q_full[g]);
     }
-    float m = __uint_as_float(kNegInf), l = 0.0f, ref = -200.0f;  // ref: log2 of the largest V scale
+    float m = __uint_as_float(kNegInf), n_log2 = m, l = 0.0f;  // largest x, x + log2(V scale); sum of 2^(x - m)
+    Bias bias;
     uint32_t nan[D / 32];
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) nan[i] = 0;
@@ -784,7 +842,6 @@ __device__ __forceinline__ void softmax_role(const Args& a, Shared* sh, uint8_t*
       tensor_fence_after();
       if (half == 0) bar_wait(&sh->tile_full[count % kTileRing], count / kTileRing & 1, patience);
       const Tile& scales = sh->tiles[count % kTileRing];
-      const float largest = scales.largest;
       const uint32_t absent = scales.absent >> 4 * half & 0xFu;
       const int seen = limit - h * kHalf;  // of this half's keys
       if (__any_sync(0xFFFFFFFFu, seen < kHalf) || absent != 0) mask_scores(half_at, seen, absent);
@@ -793,24 +850,41 @@ __device__ __forceinline__ void softmax_role(const Args& a, Shared* sh, uint8_t*
       load_begin(y, half_at + 32);
       load_end(x);
       load_end(y);
-      const float most = fmaxf(top_of(x, scales, 2 * half, factor), top_of(y, scales, 2 * half + 1, factor));
-      if (__any_sync(0xFFFFFFFFu, most > m + kRaise || largest > ref)) {
+      float tops[4], v[4];
+      top_of(x, scales, 2 * half, factor, tops);
+      top_of(y, scales, 2 * half + 1, factor, tops + 2);
+#pragma unroll
+      for (int b = 0; b < 4; ++b) v[b] = scales.v[4 * half + b];
+      const float most = largest_of(tops);
+      if (__any_sync(0xFFFFFFFFu, most > m + kRaise || term_of(tops, v) > n_log2 + kRaise)) {
+        const int stage = count % kStages;
+        bar_wait(&sh->v_full[stage], count / kStages & 1, patience);
+        const uint32_t low = filled_of(sh->filled[stage], 2 * half), high = filled_of(sh->filled[stage], 2 * half + 1);
         const float top = fmaxf(m, most);
-        const float keep_l = top == m ? 1.0f : exp2_fast(m - top);
-        if (h != 2 * begin) {  // not before the output of the half before is complete
+        if (top != m) l *= exp2_fast(m - top);
+        if (__any_sync(0xFFFFFFFFu, (low & high) != 0xFFFFFFFFu)) {
+          const float base = top == __uint_as_float(kNegInf) ? 0.0f : top;
+          set_aside(x, scales, 2 * half, factor, base, low, l);
+          set_aside(y, scales, 2 * half + 1, factor, base, high, l);
+          top_of(x, scales, 2 * half, factor, tops);
+          top_of(y, scales, 2 * half + 1, factor, tops + 2);
+        }
+        // Finite with m, also while all V is zero.
+        const float term = fmaxf(fmaxf(n_log2, term_of(tops, v)), top + kZeroLog2);
+        if (h != 2 * begin && __any_sync(0xFFFFFFFFu, term != n_log2)) {
+          // Not before the output of the half before is complete.
           bar_wait(&sh->o_done[g][half ^ 1], (turn - (half ^ 1)) & 1, patience);
           tensor_fence_after();
-          const float keep = keep_l * exp2_fast(ref - largest);
+          const float keep = term == n_log2 ? 1.0f : exp2_fast(n_log2 - term);
 #pragma unroll 1
           for (int c = 0; c < D / 8; ++c) tensor_scale8(output_at + 8 * c, keep);
         }
-        l *= keep_l;
         m = top;
-        ref = largest;
+        n_log2 = term;
+        bias.set(m, n_log2);
       }
-      const float shift = m == __uint_as_float(kNegInf) ? 0.0f : m;
-      weigh(x, scales, 2 * half, factor, shift, half_at, l);
-      weigh(y, scales, 2 * half + 1, factor, shift, half_at, l);
+      weigh(x, scales, 2 * half, factor, bias, v, half_at, l);
+      weigh(y, scales, 2 * half + 1, factor, bias, v + 2, half_at, l);
       if (work->mixed(h / 2)) {
         const int stage = count % kStages;
         bar_wait(&sh->v_full[stage], count / kStages & 1, patience);
@@ -832,9 +906,10 @@ __device__ __forceinline__ void softmax_role(const Args& a, Shared* sh, uint8_t*
 
     bar_wait(&sh->o_done[g][1], (turn - 1) & 1, patience);
     tensor_fence_after();
-    // exp2(ref) may be as small as a scale can be; a row of zero scales is zero.
+    // 2^(n - m) may be as small as a scale can be; a row of zero scales is zero.
     const bool whole = work->slot < 0;
-    const float scale = exp2_fast(ref - kWeightLog2) * (whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f);
+    const float unit = m == __uint_as_float(kNegInf) ? 0.0f : n_log2 - m;
+    const float scale = exp2_fast(unit - kWeightLog2) * (whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f);
     float* slot = whole ? nullptr : a.partial + ((int64_t)blockIdx.x * 2 + work->slot) * slot_floats(a.rows, D);
     const int row = g * kGroupRows + r;
 #pragma unroll

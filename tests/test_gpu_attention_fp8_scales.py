@@ -107,6 +107,8 @@ class Batch:
 # Up to 32 rows a KV head go to the decode kernel; contexts above 1024 keys are split over CTAs.
 FEW = [([(20, 40)], 1, 1, 128, 16, 16), ([(20, 40)], 2, 2, 64, 48, 16), ([(8, 1500)], 4, 1, 128, 16, 16),
        ([(16, 300), (3, 2100), (16, 16)], 2, 1, 64, 32, 16)]
+MANY = [([(200, 300)], 1, 1, 128, 16, 16), ([(300, 1500)], 1, 1, 128, 1024, 1024), ([(130, 1900)], 4, 1, 128, 48, 16),
+        ([(300, 400), (90, 1500)], 2, 2, 64, 32, 16)]
 
 
 def later_keys(batch, value, inside):
@@ -168,3 +170,23 @@ def check_zero_blocks(batch):
     for _, v in batch.rows:
         v.zero_()
     batch.check()
+
+
+@pytest.mark.parametrize("value,inside", [(1e4, False), (1e9, False), (1e20, False), (1e34, False), (1e9, True),
+                                          (1e20, True)])
+@pytest.mark.parametrize("lengths,q_heads,kv_heads,dim,page,block", MANY)
+def test_prompt_kernel_later_keys_of_large_values(cuda, value, inside, lengths, q_heads, kv_heads, dim, page, block):
+    batch = Batch(4, lengths, q_heads, kv_heads, dim, page, block, BF16)
+    later_keys(batch, value, inside)
+    batch.check()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("first,low", [(False, None), (True, None), (False, 4), (False, 1), (True, 4)])
+@pytest.mark.parametrize("lengths,q_heads,kv_heads,dim,page,block", MANY)
+def test_prompt_kernel_large_values_of_little_weight(cuda, dtype, first, low, lengths, q_heads, kv_heads, dim, page, block):
+    check_little_weight(5, dtype, first, low, lengths, q_heads, kv_heads, dim, page, block)
+
+
+def test_prompt_kernel_blocks_of_zeros_beside_large_values(cuda):
+    check_zero_blocks(Batch(6, [(140, 170), (100, 1600)], 4, 1, 128, 16, 16, BF16))
