@@ -65,7 +65,9 @@ KVOFF_API const char* kvoff_last_error(void);
 /*
  * Host-side fault injection for tests: the next `count` calls of entry point
  * `op` (its name without the "kvoff_" prefix, e.g. "fp8_save_blocks") fail
- * with KVOFF_EINJECTED before enqueuing any work. count = 0 clears it.
+ * with KVOFF_EINJECTED before enqueuing any work. count = 0 clears it. "attention_wait"
+ * is no entry point: in the next `count` prompt calls of kvoff_attention_fp8 waits inside
+ * the kernel give up at their first look, which kvoff_device_error then reports.
  * Replaces the reference tests' monkeypatching of torch.Tensor.copy_
  * (bench/test_cpu_prefix_cache.py:113-123, 133-143), which cannot reach
  * native copies.

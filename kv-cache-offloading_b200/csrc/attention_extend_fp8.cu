@@ -46,7 +46,11 @@
 // issues for both row tiles.
 //
 // Every wait is bounded; one that runs out sets an error flag that
-// kvoff_device_error reads; the kernel then ends without waiting for anything.
+// kvoff_device_error reads, and the kernel ends without waiting for anything but
+// its own products. What roles read from one another may be torn or stale by then:
+// it takes part in sums, but addresses, loop bounds and branches of a whole warp
+// are made of what cannot be, or are checked. The scheduler leaves a record that
+// has nothing to join.
 #include "attention_fp8.h"
 #include "codec.cuh"
 
@@ -66,7 +70,7 @@ constexpr float kRaise = 6.0f;     // log2 of how far P may pass 1
 constexpr float kWeightLog2 = 8.0f;
 constexpr float kLeastLog2 = -42.0f;  // of a V scale against 2^(n - m): P rounds to 0 in f16
 constexpr uint32_t kNegInf = 0xFF800000u;
-constexpr uint32_t kWaitNs = 1000, kMostWaits = 1u << 20;  // a second in all
+constexpr uint32_t kWaitNs = 1000;
 constexpr uint32_t kTmemColumns = 512;
 constexpr uint32_t kScoresAt = 0, kOutputsAt = 256, kGroupColumns = 128;
 constexpr int kHalf = 64;           // keys of a step: half a key tile, half a row tile's columns
@@ -141,12 +145,12 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
   __syncwarp();
   if (threadIdx.x % 32 == 0) bar_arrive(bar);
 }
-// Waits for the phase of `parity`, at most kMostWaits times kWaitNs. When that
+// Waits for the phase of `parity`, at most `most` times kWaitNs. When that
 // runs out the error flag is set and the thread goes on: what it computes then
 // means nothing, but each later wait of its ends at its first look (`most` is 0),
 // so the kernel ends, and no warp is torn apart on the way.
 struct Patience {
-  uint32_t most = kMostWaits;
+  uint32_t most;
 };
 __device__ __forceinline__ void bar_wait(uint64_t* bar, uint32_t parity, Patience& patience) {
   uint32_t done;
@@ -345,13 +349,16 @@ __device__ __forceinline__ void return_work(Shared* sh, uint32_t n) { bar_arrive
 // --- warp 18 ---------------------------------------------------------------
 
 __device__ __forceinline__ void schedule_role(const Args& a, Walk<kThreads>& walk, Shared* sh) {
-  Patience patience;
+  Patience patience{a.most_waits};
   uint32_t n = 0;
   Segment seg;
   for (bool more = true; more; ++n) {
     more = walk.next(a, &seg);
     bar_wait(&sh->work_empty[n % kWorkRing], (n / kWorkRing & 1) ^ 1, patience);
-    if (patience.most == 0) return;
+    if (patience.most == 0) {
+      walk.give_up(a);
+      return;
+    }
     Work& w = sh->work[n % kWorkRing];
     w.end = -1;
     if (more) {
@@ -405,8 +412,9 @@ struct Convert {
   // The rows of a tile that stand below `left`, zeros for the others.
   __device__ __forceinline__ void load(const uint8_t* cache, const Tile& tile, int left, uint4 (&raw)[kPasses]) const {
     const int64_t row_bytes = (int64_t)a.kv_heads * D;
-    if (tile.run) {
-      const uint8_t* at = cache + tile.place[0] + row0() * row_bytes + chunk() * 16;
+    const int64_t first = tile.place[0];
+    if (tile.run && first >= 0) {  // the page holds 128 rows from any tile's first on
+      const uint8_t* at = cache + first + row0() * row_bytes + chunk() * 16;
 #pragma unroll
       for (int i = 0; i < kPasses; ++i) {
         raw[i] = load_global(at);
@@ -492,7 +500,7 @@ __device__ __forceinline__ void convert_role(const Args& a, Shared* sh, uint8_t*
   const uint8_t* cache = is_v ? a.cache[1] : a.cache[0];
   uint64_t* full = is_v ? sh->v_full : sh->k_full;
   uint64_t* empty = is_v ? sh->v_empty : sh->k_empty;
-  Patience patience;
+  Patience patience{a.most_waits};
   uint32_t count = 0;  // key tiles so far, over all segments
   for (uint32_t n = 0;; ++n) {
     const Work* work = take_work(sh, n, patience);
@@ -535,7 +543,7 @@ __device__ __forceinline__ void tile_role(const Args& a, Shared* sh) {
   const int lane = threadIdx.x % 32;
   const int blocks = a.page / 16 / a.block_tiles;  // scale blocks of a page
   const bool long_pages = a.page % kKeyTile == 0;
-  Patience patience;
+  Patience patience{a.most_waits};
   uint32_t count = 0;
   for (uint32_t n = 0;; ++n) {
     const Work* work = take_work(sh, n, patience);
@@ -564,6 +572,7 @@ __device__ __forceinline__ void tile_role(const Args& a, Shared* sh) {
       if (count >= 2) {  // each phase in turn: a wait tells the last two apart only
         const uint32_t scores = count - 2;
         bar_wait(&sh->k_empty[scores % kStages], scores / kStages & 1, patience);
+        if (__any_sync(0xFFFFFFFFu, patience.most == 0)) return;  // the entry may still be read
       }
       Tile& t = sh->tiles[count % kTileRing];
       if (lane < 8) {
@@ -587,12 +596,12 @@ __device__ __forceinline__ void tile_role(const Args& a, Shared* sh) {
 
 // One thread for each 128-row tile g.
 template <int D>
-__device__ __forceinline__ void issue_role(Shared* sh, uint32_t base, int g) {
+__device__ __forceinline__ void issue_role(const Args& a, Shared* sh, uint32_t base, int g) {
   using L = Layout<D>;
   const uint32_t scores = sh->tmem + kScoresAt + g * kGroupColumns, output = sh->tmem + kOutputsAt + g * kGroupColumns;
   const uint32_t q = row_descriptor(base + L::kQ + g * L::kOperand);
   const uint32_t k0 = row_descriptor(base + L::kK), v0 = column_descriptor(base + L::kV);
-  Patience patience;
+  Patience patience{a.most_waits};
   uint32_t count = 0, turn = 0, segment = 0;  // key tiles so far, of the CTA and of this row tile
   for (uint32_t n = 0;; ++n) {
     const Work* work = take_work(sh, n, patience);
@@ -778,7 +787,7 @@ __device__ __forceinline__ void softmax_role(const Args& a, Shared* sh, uint8_t*
   const uint32_t scores_at = sh->tmem + lanes + kScoresAt + g * kGroupColumns;
   const uint32_t output_at = sh->tmem + lanes + kOutputsAt + g * kGroupColumns;
   const uint32_t q_at = base + L::kQ + g * L::kOperand;
-  Patience patience;
+  Patience patience{a.most_waits};
   uint32_t count = 0, turn = 0;  // key tiles so far, of the CTA and of this row tile
   for (uint32_t n = 0;; ++n) {
     const Work* work = take_work(sh, n, patience);
@@ -844,7 +853,7 @@ __device__ __forceinline__ void softmax_role(const Args& a, Shared* sh, uint8_t*
       const Tile& scales = sh->tiles[count % kTileRing];
       const uint32_t absent = scales.absent >> 4 * half & 0xFu;
       const int seen = limit - h * kHalf;  // of this half's keys
-      if (__any_sync(0xFFFFFFFFu, seen < kHalf) || absent != 0) mask_scores(half_at, seen, absent);
+      if (__any_sync(0xFFFFFFFFu, seen < kHalf || absent != 0)) mask_scores(half_at, seen, absent);
       float x[32], y[32];
       load_begin(x, half_at);
       load_begin(y, half_at + 32);
@@ -888,7 +897,7 @@ __device__ __forceinline__ void softmax_role(const Args& a, Shared* sh, uint8_t*
       if (work->mixed(h / 2)) {
         const int stage = count % kStages;
         bar_wait(&sh->v_full[stage], count / kStages & 1, patience);
-        if (*reinterpret_cast<volatile uint32_t*>(&sh->nan[stage]) == count + 1) {
+        if (__any_sync(0xFFFFFFFFu, *reinterpret_cast<volatile uint32_t*>(&sh->nan[stage]) == count + 1)) {
           const uint32_t* masks = reinterpret_cast<const uint32_t*>(smem + L::kNan + stage * L::kNanBytes) +
                                   half * kHalf * (D / 32);
           for (int i = 0; i < min(seen, kHalf); ++i)
@@ -1013,10 +1022,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_extend_fp8_kernel(const
     fewer_registers<kOtherRegisters>();
     if (warp < 18) {
       if (threadIdx.x % 32 == 0) {
-        issue_role<D>(&sh, smem_of(smem), warp - 16);
+        issue_role<D>(a, &sh, smem_of(smem), warp - 16);
         // Nothing of this CTA's is in flight when its tensor memory is freed.
         commit(&sh.drained[warp - 16]);
-        Patience patience;
+        Patience patience{kMostWaits};
         bar_wait(&sh.drained[warp - 16], 0, patience);
       }
     } else if (warp == 18) {

@@ -254,6 +254,7 @@ extern "C" int kvoff_attention_fp8(
   a.stride = c.stride;
   a.bf16 = dtype == KVOFF_BF16;
   a.wide_out = (pairs & 15u) == 0;
+  a.most_waits = c.extend && injected("attention_wait") ? 1 : attention::kMostWaits;
   a.records = static_cast<attention::Record*>(workspace);
   a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
                                        c.grid * (int64_t)sizeof(attention::Record));

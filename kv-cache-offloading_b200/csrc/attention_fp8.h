@@ -41,6 +41,7 @@ struct Args {
   int32_t stride;    // CTA c works with c + stride: kv_heads when each CTA keeps to a head, else 1
   bool bf16;
   bool wide_out;     // rows of out can be written 16 bytes at a time
+  uint32_t most_waits;       // of the prompt kernel: looks at a barrier before a wait gives up
   float* partial;            // 2 slots per CTA
   struct Record* records;    // one per CTA
 };
@@ -280,6 +281,12 @@ struct Walk {
   __device__ __forceinline__ void finish(const Args& a) const {
     if (!a.direct) a.records[cta] = record;
   }
+  // Instead of it, when the work was not done: the join must not find what stood there.
+  __device__ __forceinline__ void give_up(const Args& a) {
+    record.further = -1;
+    record.valid[0] = record.valid[1] = 0;
+    finish(a);
+  }
 };
 
 // A slot of the partial results: sums of p * v [rows, D], then each row's
@@ -355,6 +362,7 @@ int launch_extend(const Args& a, int dim, int grid, cudaStream_t stream);
 // Error flags of extend's bounded waits on the current device.
 int extend_device_error(int32_t* flags, bool clear);
 constexpr int kErrExtendWaitTimeout = 2;
+constexpr uint32_t kMostWaits = 1u << 20;  // looks of about a microsecond: a second in all
 
 }  // namespace attention
 }  // namespace kvoff
