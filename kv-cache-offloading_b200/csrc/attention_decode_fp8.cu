@@ -665,8 +665,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_decode_fp8_kernel(const
           const float2 x = *reinterpret_cast<const float2*>(from + w * (S::kWarpBytes / 4));
           sum.x += x.x;
           sum.y += x.y;
-          const float m = warp_m[w][row];
-          l += m == __uint_as_float(kNegInf) ? 0.0f : exp2_fast(m - most) * warp_l[w][row];
+          // A row that has seen nothing but NaN has no maximum, and its sum is NaN.
+          l += (most == __uint_as_float(kNegInf) ? 1.0f : exp2_fast(warp_m[w][row] - most)) * warp_l[w][row];
         }
         if (done.whole) {
           const int at = done.tile * a.rows + row;
