@@ -441,6 +441,8 @@ def _raw_stream(index: int, stream) -> int:
 
 
 _ONE_DEVICE = "the tensors must be CUDA tensors on one device"
+_NO_GRADIENT = "autograd does not see this call: use torch.no_grad(), or detach the inputs"
+_grad_enabled = torch.is_grad_enabled
 
 
 def _one_device(index: int, *tensors) -> None:
@@ -537,8 +539,15 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: tor
     the gradient of q and k from that of the result. A negative position
     leaves its token's rows unwritten, as -1 does in store_kvcache; so does one
     behind the table, which `bad_positions` (int32, CUDA) counts.
+
+    Autograd does not see the call, nor what it writes: in grad mode inputs
+    that require a gradient are refused. In an autograd.Function the backward
+    pass is the call on the gradients with `inverse`.
     """
     q_out, k_out = (q, k) if out is None else out
+    if _grad_enabled() and (q.requires_grad or k.requires_grad or table.requires_grad
+                            or q_out.requires_grad or k_out.requires_grad):
+        raise ValueError(_NO_GRADIENT)
     n, q_heads, dim = q.shape
     n_k, kv_heads, dim_k = k.shape
     if n_k != n or dim_k != dim:
@@ -620,8 +629,12 @@ def store_kvcache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Ten
     head. A call that writes a block's first token opens the block; later calls
     that need a larger scale rescale the rows that are there (see
     include/kvoff.h). Allocate the scales zeroed. One CUDA-graph-capturable
-    launch, at most 65536 tokens.
+    launch, at most 65536 tokens. Autograd does not see the call: in grad mode
+    rows that require a gradient are refused.
     """
+    if _grad_enabled() and (key.requires_grad or value.requires_grad or k_scale.requires_grad
+                            or v_scale.requires_grad):
+        raise ValueError(_NO_GRADIENT)
     shape = key.shape
     num_tokens, heads, dim = shape
     if value.shape != shape:
@@ -707,7 +720,12 @@ def attention_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     `out` and `workspace` (uint8, attention_fp8_workspace bytes) are allocated
     on the call's stream when not given; calls that may overlap need workspaces
     of their own. Enqueues at most two kernels, copies nothing to the host.
+    For inference: the result has no graph, and in grad mode inputs that
+    require a gradient are refused.
     """
+    if _grad_enabled() and (q.requires_grad or k_scale.requires_grad or v_scale.requires_grad
+                            or (out is not None and out.requires_grad)):
+        raise ValueError(_NO_GRADIENT)
     q_shape = q.shape
     n, q_heads, dim = q_shape
     index = q.get_device()
