@@ -220,8 +220,9 @@ __device__ __forceinline__ float column_most(float x) {
   return fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 16));
 }
 
-// 2^x. Past 2^126 it meets scores whose 2^(x - m) is 0 in fp32 only.
-__device__ __forceinline__ float weight_of(float x) { return exp2_fast(x > 126.0f ? 126.0f : x); }
+// scale / 2^t. What passes 2^126 is put into the scores, see kMostWeight.
+constexpr float kMostWeight = 126.0f;
+__device__ __forceinline__ float weight_of(float x) { return exp2_fast(x > kMostWeight ? kMostWeight : x); }
 
 // One warp's state over a segment.
 template <int D, int NT>
@@ -233,6 +234,7 @@ struct Rows {
   float o[kSteps][NT][4];
   float m[NT][2], l[NT][2];   // l: sum of 2^(x - m)
   float unit[NT][2];          // t: o is the sum of 2^(x - m - t) v
+  float far;                  // log2 of the largest V scale that is no more than 2^kMostWeight units of any row
 };
 
 template <int D, int NT>
@@ -301,6 +303,7 @@ __device__ __forceinline__ void load_rows(const Args& a, const Sequence& seq, co
       r.unit[j][i] = kLeastUnit;
     }
   }
+  r.far = 1e30f;
 #pragma unroll
   for (int i = 0; i < Rows<D, NT>::kSteps; ++i)
 #pragma unroll
@@ -496,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_decode_fp8_kernel(const
           const bool masked = (tile + 1) * kTile > fewest;
           const float v_log2 = scale_log2_of(scales.y);
           float weight[NT][2];  // scale / 2^t
-          bool raise = false;
+          bool raise = v_log2 > r.far;
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
             float most[2];
@@ -516,6 +519,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_decode_fp8_kernel(const
           if (__any_sync(0xFFFFFFFFu, raise)) {
             const uint32_t filled = v.filled();
             const bool some_empty = filled != 0xFFFFu;
+            float least = 1e30f;  // of the units
             const bool empty[2] = {(filled >> g & 1) == 0, (filled >> (g + 8) & 1) == 0};
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
@@ -545,12 +549,18 @@ __global__ void __launch_bounds__(kThreads, 1) attention_decode_fp8_kernel(const
                 r.m[j][k] = most;
                 r.unit[j][k] = next;
                 weight[j][k] = weight_of(v_log2 - next);
+                if (most != __uint_as_float(kNegInf)) least = fminf(least, next);
+                // The tile's scores are 2^-112 of m or less then: l does not notice.
+                const float excess = v_log2 - next - kMostWeight;
+                if (excess > 0.0f) x[j][k] += excess, x[j][k + 2] += excess;
               }
 #pragma unroll
               for (int n = 0; n < kSteps; ++n)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) r.o[n][j][k] *= keep[k & 1];
             }
+            least = fminf(least, __shfl_xor_sync(0xFFFFFFFFu, least, 1));
+            r.far = fminf(least, __shfl_xor_sync(0xFFFFFFFFu, least, 2)) + kMostWeight;
           }
           uint32_t p[NT][2], seen[NT][2];
 #pragma unroll

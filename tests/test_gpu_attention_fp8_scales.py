@@ -190,3 +190,17 @@ def test_prompt_kernel_large_values_of_little_weight(cuda, dtype, first, low, le
 
 def test_prompt_kernel_blocks_of_zeros_beside_large_values(cuda):
     check_zero_blocks(Batch(6, [(140, 170), (100, 1600)], 4, 1, 128, 16, 16, BF16))
+
+
+@pytest.mark.parametrize("lengths,q_heads,kv_heads,dim,page,block", FEW + MANY)
+def test_a_large_value_far_below_the_largest_weight(cuda, lengths, q_heads, kv_heads, dim, page, block):
+    """V is zero but for one key of 2^60 times 2^-115 of the weight: the units of weights and of terms are 2^120 apart."""
+    batch = Batch(7, lengths, q_heads, kv_heads, dim, page, block, BF16)
+    batch.q[..., 0] = 4.0
+    for (n, c), (k, v) in zip(batch.lengths, batch.rows):
+        k[..., 0] = 0.0
+        k[c // 2, :, 0] = -20.0 * dim ** 0.5  # 80 below the others' scores
+        large = v[c // 2] * 2.0 ** 60
+        v.zero_()
+        v[c // 2] = large
+    batch.check()
