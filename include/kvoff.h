@@ -357,7 +357,8 @@ KVOFF_API int kvoff_rotary(const void* q, int64_t q_stride_bytes, void* q_out,
  * are skipped; slots >= num_slots are skipped and counted into *bad_slots when
  * it is non-null (device memory). At most 65536 tokens a call. head_dim is a
  * multiple of 8 up to 256; rows are 16-byte aligned, caches 8-byte. Enqueues
- * one kernel, allocates nothing.
+ * one kernel, allocates nothing. kvoff_attention_fp8 reads fewer caches than
+ * this writes: scale blocks of 16 * 2^n tokens and heads of 64 and 128.
  */
 KVOFF_API int kvoff_store_kvcache_fp8(const void* key, int64_t key_stride_bytes,
                                       const void* value, int64_t value_stride_bytes,

@@ -7,8 +7,8 @@
 // 2 D bytes and 4 D group flops. The kernel therefore reads every byte once,
 // keeps about 160 KB of loads in flight on each SM, and spends as few
 // instructions a byte as it can. Measured: 4 sequences of 34816 keys, 32 / 8
-// heads of 128, in 59 us = 4.8 TB/s, 0.74 of a copy's rate; from 34816 to 69632
-// keys it adds 5.95 TB/s, so about 11 us of it begin and end the call (the walk
+// heads of 128, in 60 us = 4.8 TB/s, 0.73 of a copy's rate; from 34816 to 69632
+// keys it adds 45 us, so about 15 us of it begin and end the call (the walk
 // over the lengths 1.8, first addresses 1.9, first tiles 1.5, the join of the
 // warps 1.3, the join kernel 2.3 us, the launches).
 //
@@ -16,7 +16,7 @@
 //   and V in shared memory, filled by cp.async, 4 KB a tile at D = 128. No
 //   barrier of the CTA is waited for until the end of a segment. While the warps
 //   are joined there, the next segment's first tiles and its q are on their way
-//   (64 sequences of up to 8192 keys: 45.7 us instead of 47).
+//   (64 sequences of up to 8192 keys: 46.4 us; 1.3 more without).
 // * Scores: S^T[16 keys, 8 rows] = K Q^T by mma.m16n8k16 in f16. K is the M
 //   operand, so the 8 columns are the query rows of one KV head (group 4 fills
 //   half of them, group 8 all). e4m3 is a subset of f16, so K is exact; q is
@@ -61,7 +61,7 @@ static_assert(kKeyTile == kWarps * kTile, "one tile a warp and key tile");
 
 // One CTA an SM, eight warps with all the registers they can use. With two CTAs
 // at 128 registers (and half the stages each) 16 rows were spilled (138 us, now
-// 75: 4 x 34816 keys, 8 heads of 128, 12 rows) and 8 rows took 69 us, now 59. Two
+// 77: 4 x 34816 keys, 8 heads of 128, 12 rows) and 8 rows took 69 us, now 60. Two
 // tiles in one step take as long as one (60).
 template <int D, int NT>
 struct Shape {
@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_decode_fp8_kernel(const
           for (int j = 0; j < NT; ++j) {
             float most[2];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
+            for (int k = 0; k < 2; ++k) {  // scores above it raise m or t
               most[k] = r.m[j][k] + fminf(kRaise, r.unit[j][k] + (kWeightLog2 + kRaise) - v_log2);
               weight[j][k] = weight_of(v_log2 - r.unit[j][k]);
             }

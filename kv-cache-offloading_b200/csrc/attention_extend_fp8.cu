@@ -34,14 +34,15 @@
 // scores of half h + 1 are there when the softmax has done half h, so it does not
 // wait for products. Rescaling O waits for the output of the half before.
 //
-// Measured: 2048 tokens over a history of 34816 keys, 32 / 8 heads of 128, in 1.34
-// to 1.43 ms = 790 to 840 TFLOP/s, half of the rate of a plain f16 product. A
+// Measured: 2048 tokens over a history of 34816 keys, 32 / 8 heads of 128, in 1.40
+// to 1.44 ms = 790 to 810 TFLOP/s, half of the rate of a plain f16 product. A
 // softmax warp's chain of a half (wait, 64 scores out of tensor memory, maximum,
 // exponentials, P back, arrival) takes 3000 cycles where the products of both
-// row tiles take 1300. Without the exponentials the kernel takes 8 % less,
+// row tiles take 1300. Without the exponentials the kernel took 8 % less,
 // without the maximum too 12 %, without most of the products 6 %: it is the
-// latency of the chain with two such warps to a scheduler that bounds it. Tried
-// and slower: reading the scores while the half before is being weighed, one
+// latency of the chain with two such warps to a scheduler that bounds it. An n
+// for each row costs 2 to 4 % against one for the row tile, which lost a row's
+// bits to keys that it does not see. Tried and slower: reading the scores while the half before is being weighed, one
 // 128-key set of columns, all scores in registers at once, one thread that
 // issues for both row tiles.
 //

@@ -96,7 +96,10 @@ int launch_join(const Args& a, int dim, int grid, cudaStream_t stream) {
 namespace {
 
 // Longest context (in keys) that one CTA reads alone rather than sharing it:
-// the join is a second launch.
+// the join is a second launch. The host knows the tables' width and not the
+// contexts, so short contexts behind wide tables are shared too (8 heads of 128,
+// 300 keys: 1 sequence 7.4 us, with a table of 40960 keys 10.8; 4 sequences 7.6
+// and 14.7).
 constexpr int64_t kDirectKeys = 1024;
 
 struct Shape {
@@ -116,7 +119,7 @@ Choice choose(const Shape& s) {
   // The decode kernel reads the cache once for 16 rows, the prompt kernel once
   // for 256 and at the tensor cores' rate, but it takes longer to begin. Measured
   // (8 heads of 128, us, decode kernel / prompt kernel): 24 rows of 34816 keys 49
-  // / 62, 32 rows 49 / 60, 64 rows 76 / 62; 64 rows of 300 keys 10.5 / 18.4.
+  // / 60, 32 rows 49 / 59, 64 rows 76 / 61; 64 rows of 300 keys 10.7 / 18.6.
   c.extend = rows > (s.keys <= kDirectKeys ? 64 : 32);
   c.rows = c.extend ? kExtendRows : rows <= 8 ? 8 : kDecodeRows;
   c.max_tiles = (rows + c.rows - 1) / c.rows;

@@ -340,7 +340,7 @@ constexpr int kExtendRows = 256;
 // What beginning and ending a row tile costs, as keys read: 4 to 5 us of a decode
 // step, against 0.7 us a tile of 128 keys. Without it in the partition a CTA that
 // gets a hundred short sequences ends last (64 sequences of 0 to 8192 keys: 243
-// us; 512 keys 47, 768 keys 46, 1024 keys 49).
+// us; 512 keys 47, 768 keys 46, 1024 keys 49: that batch alone was measured).
 constexpr int kDecodeFixed = 768;
 constexpr int kExtendFixed = 512;
 // Raises a kernel's shared memory limit, once per kernel and device.

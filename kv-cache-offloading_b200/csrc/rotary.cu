@@ -17,16 +17,18 @@
 // cosines and sines in registers through several heads. With all heads of a
 // unit in one thread a decode step of four tokens would use a few warps only,
 // and with one head per thread every thread would load more table than data,
-// so the heads are dealt over `lanes` threads: one head each while the grid
-// is small, four once the tokens alone fill the GPU. The values are loaded
+// so the heads are dealt over `lanes` threads: one head each while there are
+// fewer threads of four heads than 2048 an SM, four from there on. The values are loaded
 // before the position is known, so one latency and not three stands between
 // them and the result.
 //
 // Measured: 16384 tokens, 64 + 8 heads of 128 bf16 in 93 us = 6.6 TB/s, a
 // copy's rate (197 us with the table row waited for first and two-byte
-// accesses to registers); 4096 tokens, 32 + 8 heads in 15.5 us; 4 tokens in
-// 2.1 us. Five heads a thread spill (30 us for the 4096 tokens), eight leave
-// too few threads (22 us).
+// accesses to registers); 4096 tokens, 32 + 8 heads in 15.4 us; 4 tokens in
+// 2.2 us. Five heads a thread spill (30 us for the 4096 tokens), eight leave
+// too few threads (22 us). 80 registers leave 768 threads an SM, so with one
+// head a thread the sizes below that border run in several rounds: 500 tokens
+// 3.7 us, 1000 5.4, 2000 9.0, 3500 17.1, where the bytes take 1.6, 3.2, 6.4 and 11.2.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -229,8 +231,9 @@ int launch(RotaryArgs a, cudaStream_t stream) {
   if (a.units > kThreads)
     return fail(KVOFF_EINVAL, "kvoff_rotary: heads of %d values at this alignment are not supported",
                 a.dim);
-  // Four heads a thread once one thread per (token, unit, 4 heads) fills the
-  // GPU; below that, as many lanes as the block has room for.
+  // Four heads a thread once the threads of four heads are 2048 an SM (2.7 times
+  // what is resident); below that, as many lanes as the block has room for. Only
+  // 4, 1023, 4096 and 16384 tokens were measured when the border was set.
   const int64_t full = (int64_t)sm_count() * 2048;
   int lanes = (heads + kUnroll - 1) / kUnroll;
   if (a.num_tokens * a.units * lanes < full) lanes = heads;

@@ -629,7 +629,8 @@ def store_kvcache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Ten
     head. A call that writes a block's first token opens the block; later calls
     that need a larger scale rescale the rows that are there (see
     include/kvoff.h). Allocate the scales zeroed. One CUDA-graph-capturable
-    launch, at most 65536 tokens. Autograd does not see the call: in grad mode
+    launch, at most 65536 tokens. attention_fp8 reads scale blocks of 16 * 2^n
+    tokens and heads of 64 and 128 only. Autograd does not see the call: in grad mode
     rows that require a gradient are refused.
     """
     if _grad_enabled() and (key.requires_grad or value.requires_grad or k_scale.requires_grad
