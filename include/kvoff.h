@@ -389,7 +389,9 @@ KVOFF_API int kvoff_store_kvcache_fp8(const void* key, int64_t key_stride_bytes,
  * tokens one another. max_seqlen_q is the longest
  * query length (it sizes the launch; the lengths themselves stay on the
  * device). Values in keys that a row does not see, NaN among them, do not
- * reach it, nor do their scales. softmax_scale is positive and finite.
+ * reach it, nor do their scales. softmax_scale is positive and finite; scores
+ * (softmax_scale * q . k) stay below 2^23 in magnitude, where fp32 tells
+ * neighbours apart.
  *
  * A row holds each key's weight times its V scale to 11 bits down to 2^-22 of
  * the largest that it meets, and to 2^-33 of it below; keys whose V is all zero

@@ -504,8 +504,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_decode_fp8_kernel(const
           for (int j = 0; j < NT; ++j) {
             float most[2];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {  // scores above it raise m or t
-              most[k] = r.m[j][k] + fminf(kRaise, r.unit[j][k] + (kWeightLog2 + kRaise) - v_log2);
+            for (int k = 0; k < 2; ++k) {  // scores above it raise m or t; not a bit higher for a large m
+              most[k] = __fadd_rd(r.m[j][k], fminf(kRaise, r.unit[j][k] + (kWeightLog2 + kRaise) - v_log2));
               weight[j][k] = weight_of(v_log2 - r.unit[j][k]);
             }
 #pragma unroll
@@ -542,10 +542,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_decode_fp8_kernel(const
                     }
                   most_filled = column_most(fmaxf(x[j][k], x[j][k + 2]));
                 }
-                const float term = most_filled + v_log2 - kWeightLog2;
+                // All against m, which may be too large for sums with t.
                 // (-inf) - (-inf) and inf - inf, of a row that has seen nothing or infinities, are none.
-                const float next = fmaxf(fmaxf(m + unit, term) - most, kLeastUnit);
-                keep[k] = most == m && next == unit ? 1.0f : exp2_fast((m + unit) - (most + next));
+                const float moved = unit + (m - most), term = (most_filled - most) + v_log2 - kWeightLog2;
+                const float next = fmaxf(fmaxf(moved, term), kLeastUnit);
+                keep[k] = most == m && next == unit ? 1.0f : exp2_fast(moved - next);
                 r.m[j][k] = most;
                 r.unit[j][k] = next;
                 weight[j][k] = weight_of(v_log2 - next);

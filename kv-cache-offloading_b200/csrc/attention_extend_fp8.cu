@@ -24,7 +24,8 @@
 // 2^(n - m) (bias in the exponent), times 2^8, and goes back to tensor memory as
 // the f16 operand of O += P V, in the place of its scores. n follows the largest
 // x + log2(scale) that the row itself has met, so its terms keep their bits
-// whatever scales other rows' keys have, or keys of no weight. Keys whose V is all
+// whatever scales other rows' keys have, or keys of no weight; it is kept as n - m,
+// since m may be too large for a sum with it. Keys whose V is all
 // zero do not count there: beside a large value, seen or not, a scale block holds
 // little else. The sum of p is taken before that, per 16 keys, and divided by the
 // same factor. m and n are raised only when they are passed by 6, so the
@@ -92,6 +93,7 @@ struct Tile {
   int64_t place[8];  // byte of the cache, at this head; negative: no page
   float k[8];
   float v[8];        // log2
+  float most_v[2];   // of each half
   uint32_t absent;   // bit g: group g has no page
   int32_t run;       // all 128 keys are read and follow one another from place[0]
 };
@@ -570,6 +572,10 @@ __device__ __forceinline__ void tile_role(const Args& a, Shared* sh) {
         v_scale = __ldg(a.scale[1] + at);
       }
       const uint32_t absent = __ballot_sync(0xFFFFFFFFu, page < 0) & 0xFFu;
+      const float v_log2 = scale_log2_of(v_scale);
+      float most = v_log2;  // of the half's four lanes
+      most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
+      most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
       if (count >= 2) {  // each phase in turn: a wait tells the last two apart only
         const uint32_t scores = count - 2;
         bar_wait(&sh->k_empty[scores % kStages], scores / kStages & 1, patience);
@@ -579,7 +585,8 @@ __device__ __forceinline__ void tile_role(const Args& a, Shared* sh) {
       if (lane < 8) {
         t.place[lane] = place;
         t.k[lane] = k_scale;
-        t.v[lane] = scale_log2_of(v_scale);
+        t.v[lane] = v_log2;
+        if (lane % 4 == 0) t.most_v[lane / 4] = most;
       }
       if (lane == 0) {
         t.absent = absent;
@@ -712,34 +719,22 @@ __device__ __forceinline__ void top_of(const float (&s)[32], const Tile& scales,
 
 __device__ __forceinline__ float largest_of(const float (&x)[4]) { return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])); }
 
-// The largest of the four groups' scores with their V scales.
-__device__ __forceinline__ float term_of(const float (&x)[4], const float (&v)[4]) {
-  return fmaxf(fmaxf(x[0] + v[0], x[1] + v[1]), fmaxf(x[2] + v[2], x[3] + v[3]));
+// The largest of the four groups' scores with their V scales, against m.
+__device__ __forceinline__ float term_of(const float (&x)[4], const float (&v)[4], float m) {
+  return fmaxf(fmaxf((x[0] - m) + v[0], (x[1] - m) + v[1]), fmaxf((x[2] - m) + v[2], (x[3] - m) + v[3]));
 }
 
-// The exponents of P: 2^(x + max(v + scaled, least)). `scaled` is 8 - n and `least`
-// kLeastLog2 + 8 - m, with m = n = 0 for a row that has seen nothing.
-struct Bias {
-  float m = 0.0f, scaled = kWeightLog2, least = kLeastLog2 + kWeightLog2;
-
-  __device__ __forceinline__ void set(float m_, float n) {
-    const bool none = m_ == __uint_as_float(kNegInf);
-    m = none ? 0.0f : m_;
-    scaled = kWeightLog2 - (none ? 0.0f : n);
-    least = kLeastLog2 + kWeightLog2 - m;
-  }
-};
-
 // P of the 32 scores of chunk c; its sums go into l. P takes the columns of
-// scores that have been read: 16 for these 32. `v`: V scales of the two groups.
-__device__ __forceinline__ void weigh(const float (&s)[32], const Tile& scales, int c, float factor, const Bias& from,
-                                      const float* v, uint32_t scores_at, float& l) {
+// scores that have been read: 16 for these 32. `v`: V scales of the two groups,
+// `unit`: n - m. The bias is rounded like a score, for P and its sum alike.
+__device__ __forceinline__ void weigh(const float (&s)[32], const Tile& scales, int c, float factor, float m,
+                                      float unit, const float* v, uint32_t scores_at, float& l) {
   uint32_t p[16];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int b = 2 * c + k;
-    const float f = factor_of(scales, b, factor), scaled = v[k] + from.scaled;
-    const float bias = scaled < from.least ? from.least : scaled;
+    const float f = factor_of(scales, b, factor), fraction = v[k] - unit;
+    const float shift = (fraction < kLeastLog2 ? kLeastLog2 : fraction) + kWeightLog2, bias = shift - m;
     float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0;
 #pragma unroll
     for (int i = 0; i < 16; i += 4) {
@@ -751,7 +746,7 @@ __device__ __forceinline__ void weigh(const float (&s)[32], const Tile& scales, 
       p[8 * k + i / 2 + 1] = pack_half(y.x, y.y);
     }
     sum0 = add_pair(sum0, sum1);
-    l = fmaf(sum0.x + sum0.y, exp2_fast(-(bias + from.m)), l);
+    l = fmaf(sum0.x + sum0.y, exp2_fast(-shift), l);
   }
   tensor_store16(scores_at + 16 * (c % 2), p);
 }
@@ -836,8 +831,9 @@ __device__ __forceinline__ void softmax_role(const Args& a, Shared* sh, uint8_t*
       tensor_fence_before();
       warp_arrive(&sh->q_full[g]);
     }
-    float m = __uint_as_float(kNegInf), n_log2 = m, l = 0.0f;  // largest x, x + log2(V scale); sum of 2^(x - m)
-    Bias bias;
+    // Largest x, and largest x + log2(V scale) against it; sum of 2^(x - m). `base` is m,
+    // 0 for a row that has seen nothing.
+    float m = __uint_as_float(kNegInf), unit = kZeroLog2, l = 0.0f, base = 0.0f;
     uint32_t nan[D / 32];
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) nan[i] = 0;
@@ -866,35 +862,33 @@ __device__ __forceinline__ void softmax_role(const Args& a, Shared* sh, uint8_t*
 #pragma unroll
       for (int b = 0; b < 4; ++b) v[b] = scales.v[4 * half + b];
       const float most = largest_of(tops);
-      if (__any_sync(0xFFFFFFFFu, most > m + kRaise || term_of(tops, v) > n_log2 + kRaise)) {
+      if (__any_sync(0xFFFFFFFFu, most > __fadd_rd(m, fminf(kRaise, unit + kRaise - scales.most_v[half])))) {
         const int stage = count % kStages;
         bar_wait(&sh->v_full[stage], count / kStages & 1, patience);
         const uint32_t low = filled_of(sh->filled[stage], 2 * half), high = filled_of(sh->filled[stage], 2 * half + 1);
         const float top = fmaxf(m, most);
         if (top != m) l *= exp2_fast(m - top);
+        base = top == __uint_as_float(kNegInf) ? 0.0f : top;
         if (__any_sync(0xFFFFFFFFu, (low & high) != 0xFFFFFFFFu)) {
-          const float base = top == __uint_as_float(kNegInf) ? 0.0f : top;
           set_aside(x, scales, 2 * half, factor, base, low, l);
           set_aside(y, scales, 2 * half + 1, factor, base, high, l);
           top_of(x, scales, 2 * half, factor, tops);
           top_of(y, scales, 2 * half + 1, factor, tops + 2);
         }
-        // Finite with m, also while all V is zero.
-        const float term = fmaxf(fmaxf(n_log2, term_of(tops, v)), top + kZeroLog2);
-        if (h != 2 * begin && __any_sync(0xFFFFFFFFu, term != n_log2)) {
+        const float moved = top == __uint_as_float(kNegInf) ? kZeroLog2 : unit + (m - top);
+        unit = fmaxf(fmaxf(moved, term_of(tops, v, top)), kZeroLog2);
+        if (h != 2 * begin && __any_sync(0xFFFFFFFFu, unit != moved)) {
           // Not before the output of the half before is complete.
           bar_wait(&sh->o_done[g][half ^ 1], (turn - (half ^ 1)) & 1, patience);
           tensor_fence_after();
-          const float keep = term == n_log2 ? 1.0f : exp2_fast(n_log2 - term);
+          const float keep = exp2_fast(moved - unit);
 #pragma unroll 1
           for (int c = 0; c < D / 8; ++c) tensor_scale8(output_at + 8 * c, keep);
         }
         m = top;
-        n_log2 = term;
-        bias.set(m, n_log2);
       }
-      weigh(x, scales, 2 * half, factor, bias, v, half_at, l);
-      weigh(y, scales, 2 * half + 1, factor, bias, v + 2, half_at, l);
+      weigh(x, scales, 2 * half, factor, base, unit, v, half_at, l);
+      weigh(y, scales, 2 * half + 1, factor, base, unit, v + 2, half_at, l);
       if (work->mixed(h / 2)) {
         const int stage = count % kStages;
         bar_wait(&sh->v_full[stage], count / kStages & 1, patience);
@@ -918,7 +912,6 @@ __device__ __forceinline__ void softmax_role(const Args& a, Shared* sh, uint8_t*
     tensor_fence_after();
     // 2^(n - m) may be as small as a scale can be; a row of zero scales is zero.
     const bool whole = work->slot < 0;
-    const float unit = m == __uint_as_float(kNegInf) ? 0.0f : n_log2 - m;
     const float scale = exp2_fast(unit - kWeightLog2) * (whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f);
     float* slot = whole ? nullptr : a.partial + ((int64_t)blockIdx.x * 2 + work->slot) * slot_floats(a.rows, D);
     const int row = g * kGroupRows + r;

@@ -28,11 +28,11 @@ def int32(values):
 
 
 def largest_terms(q, cache, scales, tables, contexts, starts, c):
-    """The largest p_t * scale_t of each row's visible keys, p the softmax, [N, Hq] in float64."""
+    """The largest p_t * scale_t and p_t of each row's visible keys, p the softmax, two [N, Hq] in float64."""
     (kc, vc), (ks, vs) = cache, scales
     page, heads = kc.shape[1], kc.shape[2]
     block, group = page // ks.shape[1], q.shape[1] // heads
-    most = torch.zeros(q.shape[:2], dtype=torch.float64, device=q.device)
+    most, weight = (torch.zeros(q.shape[:2], dtype=torch.float64, device=q.device) for _ in range(2))
     for s, context in enumerate(contexts):
         keys = torch.arange(context, device=q.device)
         at = tables[s].long()[keys // page]
@@ -46,7 +46,8 @@ def largest_terms(q, cache, scales, tables, contexts, starts, c):
                     rows = slice(h * group, (h + 1) * group)
                     p = torch.softmax(q[token, rows].double() @ k[:seen].T * c, dim=-1)
                     most[token, rows] = (p * v[:seen]).amax(-1)
-    return most
+                    weight[token, rows] = p.amax(-1)
+    return most, weight
 
 
 class Batch:
@@ -71,7 +72,7 @@ class Batch:
     def randn(self, *shape):
         return torch.randn(*shape, generator=self.g, device="cuda")
 
-    def check(self, softmax_scale=None):
+    def check(self, softmax_scale=None, exact_scores=False, v_factor=1.0):
         pages, page, heads, dim = self.shape
         c = dim ** -0.5 if softmax_scale is None else softmax_scale
         cache = [torch.zeros(self.shape, device="cuda").to(torch.float8_e4m3fn) for _ in range(2)]
@@ -80,26 +81,33 @@ class Batch:
             t = torch.arange(len(k), device="cuda")
             slots = (self.tables[s].long()[t // page] * page + t % page).int()
             ops.store_kvcache_fp8(k, v, *cache, *scales, slots)
+        scales[1] *= v_factor  # scales need not be powers of two
         contexts = [n for _, n in self.lengths]
         args = (*cache, *scales, self.tables)
         lse = torch.empty(self.q.shape[:2], device="cuda")
         got = ops.attention_fp8(self.q, *args, int32(contexts), cu_seqlens_q=int32(self.starts), lse=lse,
                                 max_seqlen_q=max(n for n, _ in self.lengths), softmax_scale=softmax_scale)
-        want, want_lse, weight, size = ref.attention(self.q, *args, contexts, self.starts, c)
-        keys = max(contexts)
+        want, want_lse, weight, size_of = ref.attention(self.q, *args, contexts, self.starts, c)
+        size = size_of
+        keys, score = max(contexts), size_of
+        most, heaviest = largest_terms(self.q, cache, scales, self.tables, contexts, self.starts, c)
+        if exact_scores:
+            # Sums of one product have no error. The exponent's error stays, but where one key has all the
+            # weight: what a weight is off by stands in the sum of weights too, and the quotient is 1.
+            size = torch.zeros_like(size)
+            score = torch.where(heaviest[..., None] == 1, 0.0, score)
         # As in attention_bound, with two differences. A weight under f16's smallest normal number is off by at
         # most 2^-25 of a unit that is 2^-8 of the row's own largest p * scale, whatever the other scales are.
         # And the exponent of a weight is a sum of scores and of logarithms of scales: six fp32 roundings of at
         # most 2^-24 of numbers up to 256 + 3 * size (log2 units).
         share = ref.half_step(FP16) + 2 * (dim + 2) * 2.0 ** -23 * size + 2.0 ** -20 + 2 * (keys + 512) * 2.0 ** -24 \
-            + 6 * math.log(2) * 2.0 ** -24 * (256 + 3 * size)
-        most = largest_terms(self.q, cache, scales, self.tables, contexts, self.starts, c)[..., None]
+            + 6 * math.log(2) * 2.0 ** -24 * (256 + 3 * score)
         bound = want.abs() * ref.half_step(self.dtype) * (1 + 2.0 ** -6) + weight * share \
-            + keys * 2.0 ** -33 * 448 * most + torch.finfo(self.dtype).smallest_normal * ref.half_step(self.dtype)
+            + keys * 2.0 ** -33 * 448 * most[..., None] + torch.finfo(self.dtype).smallest_normal * ref.half_step(self.dtype)
         off = (got.double() - want).abs()
         assert not got.isnan().any()
         assert not (off > bound).any(), f"off by {(off / bound).max():.2f} of the bound"
-        error = (dim + 2) * 2.0 ** -23 * size[..., 0] + 2.0 ** -20 + (keys + 512) * 2.0 ** -24 + 2.0 ** -20 * want_lse.abs()
+        error = (dim + 2) * 2.0 ** -23 * size_of[..., 0] + 2.0 ** -20 + (keys + 512) * 2.0 ** -24 + 2.0 ** -20 * want_lse.abs()
         fine = want_lse.isfinite()
         assert torch.equal(fine, lse.isfinite()) and ((lse.double() - want_lse).abs()[fine] <= error[fine]).all()
 
@@ -204,3 +212,20 @@ def test_a_large_value_far_below_the_largest_weight(cuda, lengths, q_heads, kv_h
         v.zero_()
         v[c // 2] = large
     batch.check()
+
+
+@pytest.mark.parametrize("q_log2,k_log2", [(3, 3), (8, 8), (12, 13), (14, 14)])
+@pytest.mark.parametrize("v_log2", [-40, 0, 30])
+@pytest.mark.parametrize("lengths,q_heads,kv_heads,dim,page,block", FEW + MANY)
+def test_large_scores(cuda, q_log2, k_log2, v_log2, lengths, q_heads, kv_heads, dim, page, block):
+    """Scores up to 2^25 (log2 units) that are exact: one key takes all the weight of the rows that see it, and the
+    others give all keys the same. Neither m nor the scale of V may lose the other's bits."""
+    batch = Batch(8, lengths, q_heads, kv_heads, dim, page, block, BF16)
+    batch.q.zero_()
+    batch.q[..., 1] = 2.0 ** q_log2
+    for (n, c), (k, v) in zip(batch.lengths, batch.rows):
+        k.zero_()
+        k[..., 1] = -2.0 ** k_log2
+        k[c - n // 2 - 1, :, 1] = 2.0 ** k_log2
+        v *= 2.0 ** v_log2
+    batch.check(exact_scores=True, v_factor=1.37)
